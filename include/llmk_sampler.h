@@ -64,6 +64,9 @@ extern "C" {
  * warn-once flag (sampler.rs:7-9, :74-76).  The engine reads NaN as -inf
  * and samples on; results for such rows are outside the parity contract. */
 #define LLMK_STATUS_NAN_LOGITS 0x10u
+/* llmk_pages_update found too few free pages for a row (out_granted says
+ * which rows were left as they were). */
+#define LLMK_STATUS_PAGES_FULL 0x20u
 
 typedef struct llmk_sampler llmk_sampler; /* opaque; owns device workspace */
 
@@ -262,6 +265,184 @@ int llmk_verify_batch(llmk_sampler* s, uint32_t batch, uint32_t vocab, const uin
                       const uint32_t* draft_tokens, const float* draft_probs,
                       uint64_t draft_stride, const float* u_accept, const float* u_resample,
                       uint32_t* out_tokens, uint32_t* out_accepted, void* hip_stream);
+
+/* Processed logits: the steps that llmk_sample_batch applies before its
+ * softmax, written out (for log-probabilities of the distribution that is
+ * sampled from, for other samplers, for speculative chains).  For row b of
+ * sequence q = row_seq[b] and every token v < vocab, in this order:
+ *   x = the logit as f32; softcap > 0: x = softcap * tanh(x / softcap);
+ *   x += the sum of the sequence's biases of v, in listing order;
+ *   n = occurrences of v in the sequence's history and the row's extra
+ *   tokens; n > 0: x = x > 0 ? x / repetition : x * repetition
+ *   (sampler.rs:128-147), x -= presence + n * frequency (mlc_parity.rs:1083);
+ *   v not allowed by the row's mask: x = -inf;
+ *   temperature > 1e-5: x /= temperature (sampler.rs:150-157).
+ * Each step is one f32 operation, as in llmk_sample_batch: without a softcap
+ * the f32 output sampled at temperature 1 with no penalties gives the tokens
+ * that the logits give with them.  The result is rounded once, to out_dtype.
+ * NaN stays NaN.  (The softcap of 16-bit logits is computed in f32 here and
+ * not rounded to 16 bits between its steps as llmk_sample_batch does.)
+ *
+ * A row whose sequence is >= sequences, whose mask_index is >= mask_rows or
+ * one of whose parameters is not finite is filled with NaN and raises
+ * LLMK_STATUS_INVALID_PARAMS. */
+typedef struct {
+  /* logits[b * row_stride + v], rows at any element offset. */
+  const void* logits;
+  int32_t dtype; /* llmk_dtype */
+  uint32_t batch;
+  uint32_t vocab;
+  uint64_t row_stride;
+  /* out[b * out_stride + v]; elements of a row past vocab are not written.
+   * out_dtype is LLMK_F32 or dtype.  In place: out = logits with the same
+   * dtype and stride; any other overlap of the rows is refused. */
+  void* out;
+  int32_t out_dtype;
+  uint64_t out_stride;
+  float softcap; /* 0 = off */
+  /* The sequence of each row, [batch]: rows of one sequence share its
+   * parameters, history and biases (a speculative chain's positions).
+   * NULL: row b is sequence b, and sequences is not read. */
+  const uint32_t* row_seq;
+  uint32_t sequences;
+  /* Per sequence; NULL = 1, 1, 0, 0 (types.rs:186-195). */
+  const float* temperature;
+  const float* repetition_penalty;
+  const float* presence_penalty;
+  const float* frequency_penalty;
+  /* Histories, indexed by sequence, in any form llmk_sample_batch_args takes:
+   * CSR, per-row buffers (hist_lengths), count tables (hist_counts).  A
+   * token's occurrences are summed modulo 2^32. */
+  const uint32_t* hist_offsets;
+  const uint32_t* hist_tokens;
+  const uint32_t* hist_lengths;
+  const uint32_t* hist_counts;
+  /* Tokens that join row b's history for this row alone (the drafts before
+   * its position): extra_tokens[extra_begin[b] .. + extra_count[b]), [batch]
+   * each; rows may share them.  NULL = none. */
+  const uint32_t* extra_begin;
+  const uint32_t* extra_count;
+  const uint32_t* extra_tokens;
+  /* Logit biases per sequence, CSR: bias_offsets[sequences + 1].  A list
+   * holds at most 2^31 pairs; ids >= vocab are ignored.  NULL = none. */
+  const uint32_t* bias_offsets;
+  const uint32_t* bias_tokens;
+  const float* bias_values;
+  /* Allow-masks, [mask_rows][mask_words_per_row] u32 as in
+   * llmk_sample_batch_args.  Row b takes row mask_index[b], none if that is
+   * negative; NULL mask_index: row b takes row b (mask_rows >= batch). */
+  const uint32_t* allow_mask;
+  uint32_t mask_words_per_row;
+  uint32_t mask_rows;
+  const int32_t* mask_index;
+} llmk_process_logits_args;
+
+/* Enqueued on hip_stream; allocates nothing and uses no workspace of the
+ * handle, whose maxima do not bound batch and vocab. */
+int llmk_process_logits(llmk_sampler* s, const llmk_process_logits_args* args,
+                        void* hip_stream);
+
+/* Log-probabilities of a batch of rows (what an OpenAI-style `logprobs`
+ * answer holds; no function of the reference has it).  With x = the logit as
+ * f32 (softcapped as in llmk_process_logits, -inf staying -inf), m = max x and S = sum
+ * exp(x - m), both held in f32: log p(v) = (x_v - m) - log S.  Tokens are
+ * ordered by (raw logit descending, index ascending); NaN is read as -inf.
+ *   out_logprobs[b] = log p(tokens[b]), out_ranks[b] = tokens before it in
+ *   the order (0: the likeliest);
+ *   out_top_ids / out_top_logprobs[b * top_n ..]: the first top_n tokens.
+ * A token with a logit of -inf has -inf, also in a row that holds nothing
+ * else; a row with a +inf logit has NaN for every other.  A token
+ * >= vocab gives NaN and rank LLMK_INVALID_TOKEN; entries of the top list
+ * past vocab are LLMK_INVALID_TOKEN and -inf. */
+typedef struct {
+  const void* logits; /* as in llmk_process_logits_args */
+  int32_t dtype;
+  uint32_t batch;
+  uint32_t vocab; /* <= 2^20 */
+  uint64_t row_stride;
+  float softcap;
+  const uint32_t* tokens; /* [batch]; NULL: the top list alone */
+  float* out_logprobs;    /* [batch], with tokens */
+  uint32_t* out_ranks;    /* [batch], with tokens; NULL: not wanted */
+  uint32_t top_n;         /* 0 .. 32 */
+  uint32_t* out_top_ids;  /* [batch][top_n] */
+  float* out_top_logprobs;
+} llmk_logprobs_args;
+
+/* Enqueued on hip_stream; allocates nothing; uses the handle's workspace
+ * (stream order, like llmk_sample_batch).  Batches above the handle's
+ * max_batch run with one workgroup per row. */
+int llmk_logprobs(llmk_sampler* s, const llmk_logprobs_args* args, void* hip_stream);
+
+/* A cache in pages: what the scheduler's block allocator keeps on the host
+ * (llm-scheduler/src/block_allocator.rs, called at scheduler.rs:162-187), on
+ * the device.  Row r holds lengths[r] tokens in the first
+ * ceil(lengths[r] / page_tokens) pages of its table row; entries behind them
+ * mean nothing and are left as they are.  refs[p] counts the rows that hold
+ * page p, and bit p & 31 of used[p >> 5] says whether any does.  All arrays
+ * are device memory of the caller; a zeroed cache is an empty one.  What the
+ * pages hold lies in n_pools pools (a layer's keys, its values, their scales,
+ * ...): page p of pool i is the pools[2 i + 1] bytes at address
+ * pools[2 i] + p * pools[2 i + 1]. */
+typedef struct {
+  uint32_t rows;        /* <= 2^20 */
+  uint32_t max_pages;   /* table entries per row */
+  uint32_t page_tokens; /* tokens per page; max_pages * page_tokens < 2^31 */
+  uint32_t num_pages;   /* <= 2^25 */
+  uint32_t* table;      /* [rows][max_pages] */
+  uint32_t* lengths;    /* [rows] */
+  uint32_t* refs;       /* [num_pages] */
+  uint32_t* used;       /* [ceil(num_pages / 32)] */
+  uint32_t* work;       /* llmk_pages_work_words words, 8-byte aligned, zeroed once */
+  uint32_t n_pools;     /* <= 65535 */
+  uint64_t page_bytes;  /* the largest pools[2 i + 1], <= 2^40 */
+  const uint64_t* pools; /* [n_pools][2], in device memory: address, bytes per page */
+} llmk_page_cache;
+
+/* The words of llmk_page_cache.work. */
+int llmk_pages_work_words(uint32_t rows, uint32_t num_pages, uint64_t* words);
+
+/* One step of a cache's rows.  parents and new_lengths: [rows], negative (or
+ * a NULL array) = nothing asked of the row.  Every row states what it asks
+ * for, and the result is that of these steps:
+ *  1. forks: row r with parent p = parents[r] begins with p's first
+ *     min(lengths[p], new_lengths[r] if >= 0) tokens: it shares their pages.
+ *     The row must be empty, and p must be another row that has no parent in
+ *     this call; p may end, shrink or grow in the same call.
+ *  2. rows longer than new_lengths shrink to it; pages no row holds any more
+ *     are free.
+ *  3. rows shorter than new_lengths grow to it, in ascending order, each new
+ *     page the lowest free one.  A row whose last page is partly filled and
+ *     shared first gets a copy of it in a page of its own (the lowest free),
+ *     unless every other row that holds it has left it so before.  From the
+ *     first row on for which too few pages are left, rows that need a page
+ *     or whose last page is shared stay as they are after steps 1 and 2.
+ * out_granted[r] = 1, or 0 for a row that did not get what it asked for: too
+ * few pages (LLMK_STATUS_PAGES_FULL), or an invalid request (a new length
+ * above max_pages * page_tokens, a row that may not fork), which changes
+ * nothing and raises LLMK_STATUS_INVALID_PARAMS.  Page contents move only
+ * for the copies of step 3.  Enqueued on hip_stream; allocates nothing; calls
+ * on one cache must not overlap. */
+int llmk_pages_update(llmk_sampler* s, const llmk_page_cache* cache, const int32_t* parents,
+                      const int32_t* new_lengths, uint32_t* out_granted, void* hip_stream);
+
+/* Moves the M pages in use to pages 0 .. M - 1: the i-th used page at or
+ * above M goes to the i-th free page below it, contents, counts and table
+ * entries; no other page moves.  out_map[p] (required, [num_pages]) = the
+ * place of page p's contents now, p for pages that did not move. */
+int llmk_pages_compact(llmk_sampler* s, const llmk_page_cache* cache, uint32_t* out_map,
+                       void* hip_stream);
+
+/* Copies page src[i] to page dst[i] in every pool, i < n: n_pools pools of
+ * num_pages pages, with page_bytes the most that a page of any has, as in
+ * llmk_page_cache.  It copies rows of anything held
+ * at a fixed pitch as well, per-row token histories and their lengths among
+ * them.  A page may be the source of several copies; the destinations must
+ * be distinct and none of them a source.  Pairs with a page >= num_pages are
+ * left out and raise LLMK_STATUS_INVALID_PARAMS. */
+int llmk_pages_copy(llmk_sampler* s, uint32_t n_pools, const uint64_t* pools,
+                    uint64_t page_bytes, uint32_t num_pages, uint32_t n, const uint32_t* src,
+                    const uint32_t* dst, void* hip_stream);
 
 /* Reads and clears the device status word (OR of LLMK_STATUS_* bits raised by
  * calls since the last read).  Synchronises `hip_stream`. */

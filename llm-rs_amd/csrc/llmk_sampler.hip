@@ -52,6 +52,7 @@
 #include <string>
 
 #include "llmk_device.h"
+#include "llmk_host.h"
 
 namespace llmk {
 
@@ -3555,35 +3556,14 @@ __global__ __launch_bounds__(WAVE) void verify_kernel(VerifyArgs v, uint32_t* st
 // ===========================================================================
 using namespace llmk;
 
-struct llmk_sampler {
-  int device;
-  uint32_t max_batch, max_vocab;
-  Ws ws;
-  void* mem;
-  size_t mem_bytes;
-  void* stage;         // aligned copies of rows passed at any offset (allocated on demand)
-  size_t stage_bytes;
-  uint32_t epoch;      // calls made (their parity picks the job count)
-  uint32_t ncu;        // the device's compute units
-  uint32_t xs_spin;    // phase 1's wait limit (LLMK_TEST_XS_SPIN at create, for tests)
-};
-
 static thread_local std::string g_last_error;
 
-static int fail(int code, const std::string& msg) {
+int llmk::fail(int code, const std::string& msg) {
   g_last_error = msg;
   return code;
 }
 
 extern "C" const char* llmk_last_error(void) { return g_last_error.c_str(); }
-
-#define HIPCHK(expr)                                                        \
-  do {                                                                      \
-    hipError_t e_ = (expr);                                                 \
-    if (e_ != hipSuccess)                                                   \
-      return fail(LLMK_ERR_HIP, std::string(#expr " failed: ") +            \
-                                    hipGetErrorString(e_));                 \
-  } while (0)
 
 static constexpr size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 

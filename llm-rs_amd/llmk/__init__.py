@@ -1,9 +1,12 @@
 """llmk — MI355X-native batched token sampling for llm-rs (HIP kernels behind a C ABI)."""
 from ._lib import LIB_PATH, EXPORTED_SYMBOLS, load  # noqa: F401
+from .pages import PageCache, PagePools  # noqa: F401
 from .sampler import (  # noqa: F401
     BatchResult,
     DeviceBatch,
     HipSampler,
+    LogitsBatch,
+    Logprobs,
     SampleParams,
     SamplerError,
     apply_top_k,

@@ -23,6 +23,7 @@ LLMK_STATUS_HISTORY_OVERFLOW = 0x2
 LLMK_STATUS_SLOT_TIMEOUT = 0x4
 LLMK_STATUS_HISTORY_FULL = 0x8
 LLMK_STATUS_NAN_LOGITS = 0x10
+LLMK_STATUS_PAGES_FULL = 0x20
 LLMK_F32 = 0
 LLMK_BF16 = 1
 LLMK_F16 = 2
@@ -41,6 +42,12 @@ EXPORTED_SYMBOLS = (
     "llmk_history_count_append",
     "llmk_sample_batch_static",
     "llmk_verify_batch",
+    "llmk_process_logits",
+    "llmk_logprobs",
+    "llmk_pages_work_words",
+    "llmk_pages_update",
+    "llmk_pages_compact",
+    "llmk_pages_copy",
 )
 
 
@@ -73,6 +80,80 @@ class SampleBatchArgs(ctypes.Structure):
         ("hist_lengths", ctypes.c_void_p),
         ("softcap", ctypes.c_float),
         ("hist_counts", ctypes.c_void_p),
+    ]
+
+
+class ProcessLogitsArgs(ctypes.Structure):
+    """Mirror of llmk_process_logits_args (include/llmk_sampler.h)."""
+
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("dtype", ctypes.c_int32),
+        ("batch", ctypes.c_uint32),
+        ("vocab", ctypes.c_uint32),
+        ("row_stride", ctypes.c_uint64),
+        ("out", ctypes.c_void_p),
+        ("out_dtype", ctypes.c_int32),
+        ("out_stride", ctypes.c_uint64),
+        ("softcap", ctypes.c_float),
+        ("row_seq", ctypes.c_void_p),
+        ("sequences", ctypes.c_uint32),
+        ("temperature", ctypes.c_void_p),
+        ("repetition_penalty", ctypes.c_void_p),
+        ("presence_penalty", ctypes.c_void_p),
+        ("frequency_penalty", ctypes.c_void_p),
+        ("hist_offsets", ctypes.c_void_p),
+        ("hist_tokens", ctypes.c_void_p),
+        ("hist_lengths", ctypes.c_void_p),
+        ("hist_counts", ctypes.c_void_p),
+        ("extra_begin", ctypes.c_void_p),
+        ("extra_count", ctypes.c_void_p),
+        ("extra_tokens", ctypes.c_void_p),
+        ("bias_offsets", ctypes.c_void_p),
+        ("bias_tokens", ctypes.c_void_p),
+        ("bias_values", ctypes.c_void_p),
+        ("allow_mask", ctypes.c_void_p),
+        ("mask_words_per_row", ctypes.c_uint32),
+        ("mask_rows", ctypes.c_uint32),
+        ("mask_index", ctypes.c_void_p),
+    ]
+
+
+class LogprobsArgs(ctypes.Structure):
+    """Mirror of llmk_logprobs_args (include/llmk_sampler.h)."""
+
+    _fields_ = [
+        ("logits", ctypes.c_void_p),
+        ("dtype", ctypes.c_int32),
+        ("batch", ctypes.c_uint32),
+        ("vocab", ctypes.c_uint32),
+        ("row_stride", ctypes.c_uint64),
+        ("softcap", ctypes.c_float),
+        ("tokens", ctypes.c_void_p),
+        ("out_logprobs", ctypes.c_void_p),
+        ("out_ranks", ctypes.c_void_p),
+        ("top_n", ctypes.c_uint32),
+        ("out_top_ids", ctypes.c_void_p),
+        ("out_top_logprobs", ctypes.c_void_p),
+    ]
+
+
+class PageCacheArgs(ctypes.Structure):
+    """Mirror of llmk_page_cache (include/llmk_sampler.h)."""
+
+    _fields_ = [
+        ("rows", ctypes.c_uint32),
+        ("max_pages", ctypes.c_uint32),
+        ("page_tokens", ctypes.c_uint32),
+        ("num_pages", ctypes.c_uint32),
+        ("table", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("refs", ctypes.c_void_p),
+        ("used", ctypes.c_void_p),
+        ("work", ctypes.c_void_p),
+        ("n_pools", ctypes.c_uint32),
+        ("page_bytes", ctypes.c_uint64),
+        ("pools", ctypes.c_void_p),
     ]
 
 
@@ -117,6 +198,18 @@ def load():
     lib.llmk_verify_batch.argtypes = [vp, u32, u32, vp, vp, u32, vp, vp, vp, u64, vp, vp, vp, vp,
                                       vp]
     lib.llmk_verify_batch.restype = ctypes.c_int
+    lib.llmk_process_logits.argtypes = [vp, ctypes.POINTER(ProcessLogitsArgs), vp]
+    lib.llmk_process_logits.restype = ctypes.c_int
+    lib.llmk_logprobs.argtypes = [vp, ctypes.POINTER(LogprobsArgs), vp]
+    lib.llmk_logprobs.restype = ctypes.c_int
+    lib.llmk_pages_work_words.argtypes = [u32, u32, ctypes.POINTER(u64)]
+    lib.llmk_pages_work_words.restype = ctypes.c_int
+    lib.llmk_pages_update.argtypes = [vp, ctypes.POINTER(PageCacheArgs), vp, vp, vp, vp]
+    lib.llmk_pages_update.restype = ctypes.c_int
+    lib.llmk_pages_compact.argtypes = [vp, ctypes.POINTER(PageCacheArgs), vp, vp]
+    lib.llmk_pages_compact.restype = ctypes.c_int
+    lib.llmk_pages_copy.argtypes = [vp, u32, vp, u64, u32, u32, vp, vp, vp]
+    lib.llmk_pages_copy.restype = ctypes.c_int
     lib.llmk_last_error.argtypes = []
     lib.llmk_last_error.restype = ctypes.c_char_p
     _lib = lib

@@ -81,6 +81,44 @@ class DeviceBatch:
     hist_counts: Optional[torch.Tensor] = None  # int32/uint32, like hist_tokens: occurrences
 
 
+@dataclass
+class LogitsBatch:
+    """Device-resident inputs of HipSampler.process_logits (torch CUDA
+    tensors; llmk_process_logits_args).  Per-sequence arrays have one entry per
+    row, or, with row_seq, per sequence."""
+
+    logits: torch.Tensor                      # [B, >=V] float32, bfloat16 or float16
+    vocab: Optional[int] = None
+    softcap: float = 0.0
+    row_seq: Optional[torch.Tensor] = None    # int32 [B]: the sequence of each row
+    temperature: Optional[torch.Tensor] = None         # float32, per sequence
+    repetition_penalty: Optional[torch.Tensor] = None
+    presence_penalty: Optional[torch.Tensor] = None
+    frequency_penalty: Optional[torch.Tensor] = None
+    hist_offsets: Optional[torch.Tensor] = None  # int32 [sequences + 1] (or [sequences])
+    hist_tokens: Optional[torch.Tensor] = None   # int32
+    hist_lengths: Optional[torch.Tensor] = None  # int32, per sequence: per-row buffers
+    hist_counts: Optional[torch.Tensor] = None   # int32, like hist_tokens: occurrences
+    extra_begin: Optional[torch.Tensor] = None   # int32 [B]
+    extra_count: Optional[torch.Tensor] = None   # int32 [B]
+    extra_tokens: Optional[torch.Tensor] = None  # int32
+    bias_offsets: Optional[torch.Tensor] = None  # int32 [sequences + 1]
+    bias_tokens: Optional[torch.Tensor] = None   # int32
+    bias_values: Optional[torch.Tensor] = None   # float32
+    allow_mask: Optional[torch.Tensor] = None    # int32 [mask rows, words]
+    mask_index: Optional[torch.Tensor] = None    # int32 [B], negative = no mask
+
+
+@dataclass
+class Logprobs:
+    """What HipSampler.logprobs returns; None for what was not asked for."""
+
+    logprobs: Optional[torch.Tensor] = None      # float32 [B]
+    ranks: Optional[torch.Tensor] = None         # int32 [B], 0 = the likeliest
+    top_ids: Optional[torch.Tensor] = None       # int32 [B, top_n]
+    top_logprobs: Optional[torch.Tensor] = None  # float32 [B, top_n]
+
+
 def _on_device(dev: torch.device, **tensors) -> None:
     """Every tensor handed to the C ABI must live on the logits' GPU: a host
     pointer or another device's pointer would reach a kernel."""
@@ -114,6 +152,82 @@ def _flat(name: str, t: Optional[torch.Tensor], dtypes) -> None:
 
 _I32 = (torch.int32,)
 _F32 = (torch.float32,)
+_U32 = _I32 + (getattr(torch, "uint32", torch.int32),)
+_DTYPES = {torch.float32: _lib.LLMK_F32, torch.bfloat16: _lib.LLMK_BF16,
+           torch.float16: _lib.LLMK_F16}
+
+
+def _logits_rows(name: str, t: torch.Tensor) -> int:
+    """The llmk_dtype of a [batch, >= vocab] tensor of logits."""
+    if t.dtype not in _DTYPES:
+        raise SamplerError(_lib.LLMK_ERR_INVALID_ARGUMENT,
+                           f"{name} must be float32, bfloat16 or float16")
+    if not _rows(t):
+        raise SamplerError(_lib.LLMK_ERR_INVALID_ARGUMENT,
+                           f"{name} must be [batch, >= vocab] with unit stride along the vocabulary")
+    return _DTYPES[t.dtype]
+
+
+def _vocab(t: torch.Tensor, vocab: Optional[int]) -> int:
+    v = t.shape[1] if vocab is None else vocab
+    if v < 0 or v > t.shape[1]:
+        raise SamplerError(_lib.LLMK_ERR_INVALID_ARGUMENT,
+                           f"vocab {v} outside the tensor's {t.shape[1]} columns")
+    return v
+
+
+def _entries(name: str, t: Optional[torch.Tensor], n: int) -> None:
+    if t is not None and t.numel() < n:
+        raise SamplerError(_lib.LLMK_ERR_INVALID_ARGUMENT,
+                           f"{name} has {t.numel()} entries, needs {n}")
+
+
+def _process_args(lb: LogitsBatch, out: torch.Tensor) -> "_lib.ProcessLogitsArgs":
+    """llmk_process_logits_args for lb, after checking every tensor's device,
+    element type, layout and length."""
+    lg = lb.logits
+    a = _lib.ProcessLogitsArgs()
+    a.dtype = _logits_rows("logits", lg)
+    a.out_dtype = _logits_rows("out", out)
+    V, B = _vocab(lg, lb.vocab), lg.shape[0]
+    if out.shape[0] != B or out.shape[1] < V:
+        raise SamplerError(_lib.LLMK_ERR_INVALID_ARGUMENT, "out must be [batch, >= vocab]")
+    floats = ("temperature", "repetition_penalty", "presence_penalty", "frequency_penalty")
+    ints = ("row_seq", "hist_offsets", "hist_tokens", "hist_lengths", "hist_counts", "extra_begin",
+            "extra_count", "extra_tokens", "bias_offsets", "bias_tokens", "mask_index")
+    fields = {n: getattr(lb, n) for n in floats + ints + ("bias_values", "allow_mask")}
+    _on_device(lg.device, out=out, **fields)
+    for n in floats + ("bias_values",):
+        _flat(n, fields[n], _F32)
+    for n in ints + ("allow_mask",):
+        _flat(n, fields[n], _U32 if n != "mask_index" else _I32)
+    # the sequences: as many as every array that is per sequence has entries for
+    per_seq = [fields[n].numel() for n in floats + ("hist_lengths",) if fields[n] is not None]
+    if lb.hist_offsets is not None:
+        per_seq.append(lb.hist_offsets.numel() - (0 if lb.hist_lengths is not None else 1))
+    if lb.bias_offsets is not None:
+        per_seq.append(lb.bias_offsets.numel() - 1)
+    seqs = max(0, min(per_seq)) if per_seq else (B if lb.row_seq is None else 2**31 - 1)
+    if lb.row_seq is None and seqs < B:
+        raise SamplerError(_lib.LLMK_ERR_INVALID_ARGUMENT,
+                           f"per-row arrays for {seqs} rows, the logits have {B}")
+    for n in ("row_seq", "extra_begin", "extra_count", "mask_index"):
+        _entries(n, fields[n], B)
+    if lb.hist_counts is not None and lb.hist_tokens is not None:
+        _entries("hist_counts", lb.hist_counts, lb.hist_tokens.numel())
+    if lb.bias_tokens is not None and lb.bias_values is not None:
+        _entries("bias_values", lb.bias_values, lb.bias_tokens.numel())
+    if lb.allow_mask is not None and lb.allow_mask.dim() != 2:
+        raise SamplerError(_lib.LLMK_ERR_INVALID_ARGUMENT, "allow_mask must be [rows, words]")
+    a.logits, a.batch, a.vocab, a.row_stride = lg.data_ptr(), B, V, _row_stride(lg)
+    a.out, a.out_stride = out.data_ptr(), _row_stride(out)
+    a.softcap = float(lb.softcap or 0.0)
+    a.sequences = seqs
+    for n, t in fields.items():
+        setattr(a, n, _ptr(t))
+    if lb.allow_mask is not None:
+        a.mask_rows, a.mask_words_per_row = lb.allow_mask.shape
+    return a
 
 
 def _batch_args(db: DeviceBatch, out_tokens: torch.Tensor,
@@ -433,6 +547,79 @@ class HipSampler:
         if rc != 0:
             raise SamplerError(rc, _lib.last_error())
         return tok, acc
+
+    # ---- operators on logits ----------------------------------------------
+    def _same_device(self, dev: torch.device) -> None:
+        if dev.type != "cuda" or dev.index != self.device:
+            raise SamplerError(_lib.LLMK_ERR_INVALID_ARGUMENT,
+                               f"tensors on {dev}, the sampler on cuda:{self.device}")
+
+    def process_logits(self, lb: LogitsBatch, out: Optional[torch.Tensor] = None,
+                       stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
+        """llmk_process_logits: softcap, logit bias, penalties, allow-mask and
+        temperature of every row, into `out` ([B, >= V], float32 or the logits'
+        dtype; lb.logits itself: in place), by default a new float32 tensor."""
+        if out is None:
+            _logits_rows("logits", lb.logits)
+            out = torch.empty(lb.logits.shape[0], _vocab(lb.logits, lb.vocab), dtype=torch.float32,
+                              device=lb.logits.device)
+        a = _process_args(lb, out)
+        self._same_device(lb.logits.device)
+        rc = self._lib.llmk_process_logits(
+            self._h, ctypes.byref(a), ctypes.c_void_p(self._stream(lb.logits, stream).cuda_stream))
+        if rc != 0:
+            raise SamplerError(rc, _lib.last_error())
+        return out
+
+    def logprobs(self, logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
+                 top_n: int = 0, softcap: float = 0.0, vocab: Optional[int] = None,
+                 stream: Optional[torch.cuda.Stream] = None) -> Logprobs:
+        """llmk_logprobs: log-probability and rank of tokens[b] in row b, and
+        the row's top_n likeliest tokens (ties: the lower id first)."""
+        a = _lib.LogprobsArgs()
+        a.dtype = _logits_rows("logits", logits)
+        _on_device(logits.device, tokens=tokens)
+        _flat("tokens", tokens, _U32)
+        self._same_device(logits.device)
+        B, dev = logits.shape[0], logits.device
+        _entries("tokens", tokens, B)
+        if not 0 <= int(top_n) <= 32:
+            raise SamplerError(_lib.LLMK_ERR_CAPACITY, "top_n outside 0 .. 32")
+        r = Logprobs()
+        if tokens is not None:
+            r.logprobs = torch.empty(B, dtype=torch.float32, device=dev)
+            r.ranks = torch.empty(B, dtype=torch.int32, device=dev)
+        if top_n:
+            r.top_ids = torch.empty(B, top_n, dtype=torch.int32, device=dev)
+            r.top_logprobs = torch.empty(B, top_n, dtype=torch.float32, device=dev)
+        a.logits, a.batch, a.vocab = logits.data_ptr(), B, _vocab(logits, vocab)
+        a.row_stride, a.softcap = _row_stride(logits), float(softcap or 0.0)
+        a.tokens, a.out_logprobs, a.out_ranks = _ptr(tokens), _ptr(r.logprobs), _ptr(r.ranks)
+        a.top_n, a.out_top_ids, a.out_top_logprobs = top_n, _ptr(r.top_ids), _ptr(r.top_logprobs)
+        st = self._stream(logits, stream)
+        rc = self._lib.llmk_logprobs(self._h, ctypes.byref(a), ctypes.c_void_p(st.cuda_stream))
+        if rc != 0:
+            raise SamplerError(rc, _lib.last_error())
+        self._keep(st, *[t for t in (r.logprobs, r.ranks, r.top_ids, r.top_logprobs) if t is not None])
+        return r
+
+    def copy_pages(self, pools: "PagePools", src: torch.Tensor, dst: torch.Tensor,
+                   stream: Optional[torch.cuda.Stream] = None) -> None:
+        """llmk_pages_copy: page src[i] to page dst[i] in every pool.  The
+        destinations must be distinct, and none of them a source."""
+        _on_device(pools.addresses.device, src=src, dst=dst)
+        _flat("src", src, _U32)
+        _flat("dst", dst, _U32)
+        self._same_device(pools.addresses.device)
+        if src.numel() != dst.numel():
+            raise SamplerError(_lib.LLMK_ERR_INVALID_ARGUMENT, "src and dst differ in length")
+        st = self._stream(src, stream)
+        rc = self._lib.llmk_pages_copy(self._h, pools.count, _ptr(pools.addresses),
+                                       pools.page_bytes, pools.num_pages, src.numel(),
+                                       src.data_ptr(), dst.data_ptr(),
+                                       ctypes.c_void_p(st.cuda_stream))
+        if rc != 0:
+            raise SamplerError(rc, _lib.last_error())
 
     # ---- the per-row reference call (LlmBackend::sample) ------------------
     def sample(self, logits: torch.Tensor, params: SampleParams,

@@ -38,6 +38,7 @@ pub const LLMK_STATUS_HISTORY_OVERFLOW: u32 = 0x2;
 pub const LLMK_STATUS_SLOT_TIMEOUT: u32 = 0x4;
 pub const LLMK_STATUS_HISTORY_FULL: u32 = 0x8;
 pub const LLMK_STATUS_NAN_LOGITS: u32 = 0x10;
+pub const LLMK_STATUS_PAGES_FULL: u32 = 0x20;
 
 /// `llmk_sample_batch_args`, field for field.  Null pointers select the
 /// `SampleParams` defaults (llm-core/src/types.rs:186-195) or switch the
@@ -115,6 +116,98 @@ impl Default for LlmkSampleBatchArgs {
     }
 }
 
+/// `llmk_process_logits_args`, field for field: null pointers switch a step
+/// off.  `LlmkProcessLogitsArgs::zeroed()` is an args struct with every
+/// optional input off.
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct LlmkProcessLogitsArgs {
+    pub logits: *const c_void,
+    pub dtype: i32,
+    pub batch: u32,
+    pub vocab: u32,
+    pub row_stride: u64,
+    /// `logits` with the same dtype and stride: in place.
+    pub out: *mut c_void,
+    pub out_dtype: i32,
+    pub out_stride: u64,
+    pub softcap: f32,
+    /// The sequence of each row (null: row b is sequence b).
+    pub row_seq: *const u32,
+    pub sequences: u32,
+    pub temperature: *const f32,
+    pub repetition_penalty: *const f32,
+    pub presence_penalty: *const f32,
+    pub frequency_penalty: *const f32,
+    pub hist_offsets: *const u32,
+    pub hist_tokens: *const u32,
+    pub hist_lengths: *const u32,
+    pub hist_counts: *const u32,
+    pub extra_begin: *const u32,
+    pub extra_count: *const u32,
+    pub extra_tokens: *const u32,
+    pub bias_offsets: *const u32,
+    pub bias_tokens: *const u32,
+    pub bias_values: *const f32,
+    pub allow_mask: *const u32,
+    pub mask_words_per_row: u32,
+    pub mask_rows: u32,
+    pub mask_index: *const i32,
+}
+
+impl LlmkProcessLogitsArgs {
+    pub fn zeroed() -> Self {
+        // SAFETY: every field is an integer, a float or a raw pointer.
+        unsafe { std::mem::zeroed() }
+    }
+}
+
+/// `llmk_logprobs_args`, field for field.
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct LlmkLogprobsArgs {
+    pub logits: *const c_void,
+    pub dtype: i32,
+    pub batch: u32,
+    pub vocab: u32,
+    pub row_stride: u64,
+    pub softcap: f32,
+    pub tokens: *const u32,
+    pub out_logprobs: *mut f32,
+    pub out_ranks: *mut u32,
+    pub top_n: u32,
+    pub out_top_ids: *mut u32,
+    pub out_top_logprobs: *mut f32,
+}
+
+impl LlmkLogprobsArgs {
+    pub fn zeroed() -> Self {
+        // SAFETY: every field is an integer, a float or a raw pointer.
+        unsafe { std::mem::zeroed() }
+    }
+}
+
+/// `llmk_page_cache`, field for field: the device form of the scheduler's
+/// block allocator (llm-scheduler/src/block_allocator.rs).
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub struct LlmkPageCache {
+    pub rows: u32,
+    pub max_pages: u32,
+    pub page_tokens: u32,
+    pub num_pages: u32,
+    pub table: *mut u32,
+    pub lengths: *mut u32,
+    pub refs: *mut u32,
+    pub used: *mut u32,
+    /// `pages_work_words` words, zeroed once.
+    pub work: *mut u32,
+    pub n_pools: u32,
+    pub page_bytes: u64,
+    /// `[n_pools][2]` in device memory: address, bytes per page.
+    pub pools: *const u64,
+}
+
 /// The opaque `llmk_sampler`.
 #[repr(C)]
 pub struct LlmkSampler {
@@ -149,6 +242,19 @@ extern "C" {
                              draft_stride: u64, u_accept: *const f32, u_resample: *const f32,
                              out_tokens: *mut u32, out_accepted: *mut u32,
                              hip_stream: *mut c_void) -> c_int;
+    pub fn llmk_process_logits(s: *mut LlmkSampler, args: *const LlmkProcessLogitsArgs,
+                               hip_stream: *mut c_void) -> c_int;
+    pub fn llmk_logprobs(s: *mut LlmkSampler, args: *const LlmkLogprobsArgs,
+                         hip_stream: *mut c_void) -> c_int;
+    pub fn llmk_pages_work_words(rows: u32, num_pages: u32, words: *mut u64) -> c_int;
+    pub fn llmk_pages_update(s: *mut LlmkSampler, cache: *const LlmkPageCache,
+                             parents: *const i32, new_lengths: *const i32,
+                             out_granted: *mut u32, hip_stream: *mut c_void) -> c_int;
+    pub fn llmk_pages_compact(s: *mut LlmkSampler, cache: *const LlmkPageCache,
+                              out_map: *mut u32, hip_stream: *mut c_void) -> c_int;
+    pub fn llmk_pages_copy(s: *mut LlmkSampler, n_pools: u32, pools: *const u64,
+                           page_bytes: u64, num_pages: u32, n: u32, src: *const u32,
+                           dst: *const u32, hip_stream: *mut c_void) -> c_int;
     pub fn llmk_sampler_status(s: *mut LlmkSampler, hip_stream: *mut c_void,
                                status: *mut u32) -> c_int;
     pub fn llmk_sampler_destroy(s: *mut LlmkSampler);
@@ -285,6 +391,57 @@ impl HipSampler {
                                 out_tokens, out_accepted, stream))
     }
 
+    /// Processed logits (softcap, logit bias, penalties, allow-mask,
+    /// temperature), as `llmk_process_logits` documents.
+    ///
+    /// # Safety
+    /// As `sample_batch`.
+    pub unsafe fn process_logits(&self, args: &LlmkProcessLogitsArgs, stream: *mut c_void)
+        -> Result<(), LlmkError> {
+        check(llmk_process_logits(self.raw, args, stream))
+    }
+
+    /// Log-probabilities and ranks of one token per row, and the likeliest
+    /// tokens.
+    ///
+    /// # Safety
+    /// As `sample_batch`.
+    pub unsafe fn logprobs(&self, args: &LlmkLogprobsArgs, stream: *mut c_void)
+        -> Result<(), LlmkError> {
+        check(llmk_logprobs(self.raw, args, stream))
+    }
+
+    /// One step of a paged cache's rows: forks, ends and growth.
+    ///
+    /// # Safety
+    /// `cache`'s arrays as documented; `parents` and `new_lengths` null or
+    /// `rows` entries, `out_granted` `rows` entries, on the device.
+    pub unsafe fn pages_update(&self, cache: &LlmkPageCache, parents: *const i32,
+                               new_lengths: *const i32, out_granted: *mut u32,
+                               stream: *mut c_void) -> Result<(), LlmkError> {
+        check(llmk_pages_update(self.raw, cache, parents, new_lengths, out_granted, stream))
+    }
+
+    /// Moves the pages in use to the front.
+    ///
+    /// # Safety
+    /// As `pages_update`; `out_map` has `num_pages` entries.
+    pub unsafe fn pages_compact(&self, cache: &LlmkPageCache, out_map: *mut u32,
+                                stream: *mut c_void) -> Result<(), LlmkError> {
+        check(llmk_pages_compact(self.raw, cache, out_map, stream))
+    }
+
+    /// Copies page `src[i]` to page `dst[i]` in every pool.
+    ///
+    /// # Safety
+    /// Device arrays; pools of `num_pages` pages of `page_bytes` bytes.
+    #[allow(clippy::too_many_arguments)]
+    pub unsafe fn pages_copy(&self, n_pools: u32, pools: *const u64, page_bytes: u64,
+                             num_pages: u32, n: u32, src: *const u32, dst: *const u32,
+                             stream: *mut c_void) -> Result<(), LlmkError> {
+        check(llmk_pages_copy(self.raw, n_pools, pools, page_bytes, num_pages, n, src, dst, stream))
+    }
+
     /// Reads and clears the device status word (`LLMK_STATUS_*` bits raised
     /// since the last read); synchronises `stream`.
     pub fn status(&self, stream: *mut c_void) -> Result<u32, LlmkError> {
@@ -318,6 +475,14 @@ impl Drop for HipSampler {
 pub unsafe fn sample_batch_static(args: &LlmkSampleBatchArgs, status: *mut u32,
                                   stream: *mut c_void) -> Result<(), LlmkError> {
     check(llmk_sample_batch_static(args, status, stream))
+}
+
+/// The words of `LlmkPageCache::work`.
+pub fn pages_work_words(rows: u32, num_pages: u32) -> Result<u64, LlmkError> {
+    let mut words = 0u64;
+    // SAFETY: `words` is a valid out-pointer.
+    check(unsafe { llmk_pages_work_words(rows, num_pages, &mut words) })?;
+    Ok(words)
 }
 
 /// `SampleParams::top_k` (a `usize`, types.rs:181) as the engine's `i32`:
