@@ -315,14 +315,12 @@ struct LArgs {
   uint32_t* out_ids;
   float* out_top;
   uint32_t* arrive;  // [B]
-  f2v* part;         // [B][G]: max, sum
-  u2v* cand;         // [B * G][CAND_CAP]: (rank count, -), then the segment's top list
+  float* tmax;       // [B][2 * MAX_SLOTS]: the tiles' maxima
+  uint32_t* part;    // [B * G][4]: m, s, tokens before the chosen one
 };
 
-constexpr uint32_t LT = 256, LWAVES = LT / WAVE;
-constexpr uint32_t TOP_MAX = 32;   // largest top_n
-constexpr uint32_t TLIST = 256;    // candidates of a wave
-constexpr uint32_t TMERGE = 512;   // candidates of a row's segments: G * top_n
+constexpr uint32_t TOP_MAX = 32;  // largest top_n
+constexpr uint32_t TLIST = 256;   // candidates of a wave
 
 // A token's place in the order (logit descending, index ascending) as a
 // number that falls along it; no token has 0.
@@ -363,18 +361,19 @@ __device__ __forceinline__ uint32_t keep_first(LDS uint64_t* list, uint32_t m, u
   return umin(m, n);
 }
 
-// The n-th largest of the lanes' order-preserving keys (n <= 64), by bits.
-template <int Q>
-__device__ __forceinline__ uint32_t nth_key(const uint32_t (&key)[Q], uint32_t n) {
-  uint32_t t = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t c = t | (1u << bit);
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < Q; ++i) m += (uint32_t)__popcll(__ballot(key[i] >= c));
-    if (m >= n) t = c;
-  }
-  return t;
+template <int DT>
+__device__ __forceinline__ float raw_logit(const void* row, uint32_t e) {
+  const float x = Elem<DT>::SZ == 4 ? G((const float*)row)[e]
+                                    : cvt16<DT>(G((const uint16_t*)row)[e]);
+  return x == x ? x : NEG_INF;
+}
+
+// Words passed between workgroups, at agent scope.
+__device__ __forceinline__ void put_agent(uint32_t* p, uint32_t v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint32_t get_agent(const uint32_t* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 constexpr float kLog2e = 0x1.715476p+0f;
@@ -382,108 +381,96 @@ __device__ __forceinline__ float exp_diff(float x, float m) {  // e^(x - m), x <
   return __builtin_amdgcn_exp2f((x - m) * kLog2e);
 }
 
-// One workgroup per (row, segment): four waves, each with every fourth
-// 1024-logit tile of the segment.  A lane keeps the running maximum m and sum
-// s = sum e^(x - m) of its logits; the wave keeps its first top_n tokens in
-// order in LDS: a tile whose maximum does not pass the last of them is done
-// with, and only tiles that hold a new one look at single logits.  The first
-// tile starts from the top_n-th largest of the lanes' maxima, below which no
-// logit of the tile can belong to the list.
-template <int DT, bool TOP>
-__global__ __launch_bounds__(LT) void logprobs_kernel(LArgs a) {
-  __shared__ uint64_t s_list[LWAVES * TLIST];
-  __shared__ float s_m[LWAVES], s_s[LWAVES];
-  __shared__ uint32_t s_c[LWAVES], s_n[LWAVES], s_last;
-  constexpr uint32_t W = Elem<DT>::W, NP = 16 / W;
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, wv = tid >> 6;
-  const uint32_t b = blockIdx.x / a.G, g = blockIdx.x % a.G;
-  const void* row = (const char*)a.logits + (uint64_t)b * a.stride * Elem<DT>::SZ;
-  const uint32_t t0 = g * a.tps, t1 = umin(t0 + a.tps, a.ntiles);
-  LDS uint64_t* list = (LDS uint64_t*)s_list + wv * TLIST;
-
+// The 1024 logits of a tile, 16 a lane: raw bits, and element i's index.
+template <int DT>
+struct Tile16 {
+  static constexpr uint32_t W = Elem<DT>::W, NP = 16 / W;
   u4v raw[NP];
-  auto request = [&](uint32_t t) {
+  __device__ __forceinline__ void request(const void* row, uint32_t t, uint32_t V) {
 #pragma unroll
     for (uint32_t j = 0; j < NP; ++j) {
-      const uint32_t e = t * TILE + (j * 64 + lane) * W;
+      const uint32_t e = t * TILE + (j * 64 + (threadIdx.x & 63u)) * W;
       raw[j] = u4v{0, 0, 0, 0};
-      if (e < a.V) raw[j] = load_pack<DT>(row, e, a.V);
+      if (e < V) raw[j] = load_pack<DT>(row, e, V);
     }
-  };
-  uint32_t t = t0 + wv;
-  if (t < t1) request(t);
-  const uint32_t tok = a.tokens ? G(a.tokens)[b] : EMPTY;
-  const bool chosen = tok < a.V;
-  auto raw_logit = [&](uint32_t e) {
-    const float x = Elem<DT>::SZ == 4 ? G((const float*)row)[e]
-                                      : cvt16<DT>(G((const uint16_t*)row)[e]);
-    return x == x ? x : NEG_INF;
-  };
-  const float lt = chosen ? raw_logit(tok) : __builtin_huge_valf();
-
-  float m = NEG_INF, s = 0.0f;
-  uint32_t before = 0, held = 0;
-  float bar = NEG_INF;  // the value the list's last token has, once it is full
-  bool full = false;
-  for (; t < t1; t += LWAVES) {
-    float x[16];
+  }
+  static __device__ __forceinline__ uint32_t index(uint32_t t, uint32_t i) {
+    return t * TILE + ((i / W) * 64 + (threadIdx.x & 63u)) * W + i % W;
+  }
+  // as floats, NaN and what lies past V as -inf
+  __device__ __forceinline__ void values(uint32_t t, uint32_t V, float (&x)[16]) const {
 #pragma unroll
     for (uint32_t i = 0; i < 16; ++i) {
       x[i] = unpack<DT>(raw[i / W], i % W);
       if (!(x[i] == x[i])) x[i] = NEG_INF;
     }
-    const uint32_t base = t * TILE;
-    auto index = [&](uint32_t i) { return base + ((i / W) * 64 + lane) * W + i % W; };
-    if (base + TILE > a.V) {
+    if (t * TILE + TILE > V) {
 #pragma unroll
       for (uint32_t i = 0; i < 16; ++i)
-        if (index(i) >= a.V) x[i] = NEG_INF;
+        if (index(t, i) >= V) x[i] = NEG_INF;
     }
-    if (t + LWAVES < t1) request(t + LWAVES);
+  }
+};
+
+// One workgroup per (row, segment), its waves taking the segment's 1024-logit
+// tiles in turn.  A lane keeps the running maximum m and sum s = sum e^(x - m)
+// of its logits and how many come before the chosen token; the wave leaves
+// each tile's maximum.  The row's last workgroup joins the segments.
+//
+// The likeliest tokens lie in the top_n tiles that are first by (maximum
+// descending, index ascending): a token of any other tile has the top_n
+// maxima of those before it.  So the stream carries no list; the last
+// workgroup reads top_n tiles again and picks from them.  (A list of
+// candidates kept by every wave took 90 us instead of 31 for 256 x 151936 f32
+// with a list of 8.)
+//
+// Bound by HBM: that call reads its 156 MB at 5.0 TB/s, without a list at 5.5
+// TB/s.  64 registers, so that 8 waves fit a SIMD (2047 x 32000 f16 with a
+// list of 1: 35 us with 80 registers, 31.6 with 64); the last steps are kept in
+// short loops, since their code comes from L2 when a workgroup first gets there.
+template <int DT, bool TOP, uint32_t LT>
+__global__ __launch_bounds__(LT, 8) void logprobs_kernel(LArgs a) {
+  constexpr uint32_t LWAVES = LT / WAVE;
+  __shared__ uint64_t s_list[TOP ? LWAVES * TLIST : 1];
+  __shared__ float s_tmax[TOP ? MAX_TILES : 1];
+  __shared__ float s_m[LWAVES], s_s[LWAVES];
+  __shared__ uint32_t s_c[LWAVES], s_n[LWAVES], s_sel[TOP_MAX], s_last, s_count, s_bound;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wv = tid >> 6;
+  const uint32_t b = blockIdx.x / a.G, g = blockIdx.x % a.G;
+  const void* row = (const char*)a.logits + (uint64_t)b * a.stride * Elem<DT>::SZ;
+  const uint32_t t0 = g * a.tps, t1 = umin(t0 + a.tps, a.ntiles);
+
+  Tile16<DT> in;
+  uint32_t t = t0 + wv;
+  if (t < t1) in.request(row, t, a.V);
+  const uint32_t tok = a.tokens ? G(a.tokens)[b] : EMPTY;
+  const bool chosen = tok < a.V;
+  const float lt = chosen ? raw_logit<DT>(row, tok) : __builtin_huge_valf();
+
+  float m = NEG_INF, s = 0.0f;
+  uint32_t before = 0;
+  for (; t < t1; t += LWAVES) {
+    float x[16];
+    in.values(t, a.V, x);
+    if (t + LWAVES < t1) in.request(row, t + LWAVES, a.V);
     float mx = x[0];
 #pragma unroll
     for (uint32_t i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
-    // tokens before the chosen one
+    if (TOP) {
+      const float w = wave_max(mx);
+      if (lane == 0) s_tmax[t - t0] = w;
+    }
     if (chosen) {
-      if (base + TILE <= tok) {
+      if (t * TILE + TILE <= tok) {
 #pragma unroll
         for (uint32_t i = 0; i < 16; ++i) before += x[i] >= lt ? 1u : 0u;
-      } else if (base > tok) {
+      } else if (t * TILE > tok) {
 #pragma unroll
         for (uint32_t i = 0; i < 16; ++i) before += x[i] > lt ? 1u : 0u;
       } else {
 #pragma unroll
         for (uint32_t i = 0; i < 16; ++i)
-          before += x[i] > lt || (x[i] == lt && index(i) < tok) ? 1u : 0u;
-      }
-    }
-    if (TOP) {
-      if (!full || __any(mx > bar)) {
-        float least = bar;
-        if (!full) {
-          const uint32_t k[1] = {fkey(mx + 0.0f)};
-          least = funkey(nth_key<1>(k, a.top_n));
-        }
-        // Entries equal to the bar are taken along: within the tile an equal
-        // one may come earlier in the order.
-#pragma unroll
-        for (uint32_t i = 0; i < 16; ++i) {
-          const bool take = x[i] >= least && index(i) < a.V;
-          const uint64_t who = __ballot(take);
-          if (who) {
-            if (take) list[held + lanes_below(who)] = order_key(x[i], index(i));
-            held += (uint32_t)__popcll(who);
-            if (held > TLIST - 64) {
-              held = keep_first<TLIST / 64>(list, held, a.top_n);
-              if (held == a.top_n) least = key_value(list[a.top_n - 1]);
-            }
-          }
-        }
-        if (!full || held > a.top_n + 16) {
-          held = keep_first<TLIST / 64>(list, held, a.top_n);
-          full = held == a.top_n;
-          if (full) bar = key_value(list[a.top_n - 1]);
-        }
+          before += x[i] > lt || (x[i] == lt && Tile16<DT>::index(t, i) < tok) ? 1u : 0u;
       }
     }
     if (DT & SOFTCAP) {
@@ -510,109 +497,65 @@ __global__ __launch_bounds__(LT) void logprobs_kernel(LArgs a) {
   const float wm = wave_max(m);
   s = wave_tree_sum(m == NEG_INF ? 0.0f : s * exp_diff(m, wm));
   before = bcast63u(wave_incl_scan(before));
-  if (TOP) held = keep_first<TLIST / 64>(list, held, a.top_n);
   if (lane == 0) {
     s_m[wv] = wm;
     s_s[wv] = s;
     s_c[wv] = before;
-    s_n[wv] = held;
+  }
+  if (TOP) {
+    if (tid == 0) s_count = 0;
+    s_list[tid] = 0;
+    if (tid < 4) s_list[LT + tid] = 0;
   }
   __syncthreads();
-  if (wv != 0 && a.G == 1) return;
-  float M = NEG_INF, S = 0.0f;
-  uint32_t C = 0, N = 0;
-  LDS uint64_t* all = (LDS uint64_t*)s_list;
-  if (wv == 0) {
+  float M = s_m[0], S = 0.0f;
+  uint32_t C = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < LWAVES; ++i) {
-      M = fmaxf(M, s_m[i]);
-      C += s_c[i];
-    }
+  for (uint32_t i = 1; i < LWAVES; ++i) M = fmaxf(M, s_m[i]);
 #pragma unroll
-    for (uint32_t i = 0; i < LWAVES; ++i)
-      if (s_m[i] != NEG_INF) S += s_s[i] * exp_diff(s_m[i], M);
-    if (TOP) {
-      // the waves' lists end to end (each moves down, none past its own start)
-      N = s_n[0];
-      for (uint32_t i = 1; i < LWAVES; ++i) {
-        const uint32_t ni = s_n[i];
-        const uint64_t k = lane < ni ? all[i * TLIST + lane] : 0u;
-        wave_sync();
-        if (lane < ni) all[N + lane] = k;
-        N += ni;
-      }
-      N = keep_first<LWAVES * TOP_MAX / 64>(all, N, a.top_n);
-    }
+  for (uint32_t i = 0; i < LWAVES; ++i) {
+    if (s_m[i] != NEG_INF) S += s_s[i] * exp_diff(s_m[i], M);
+    C += s_c[i];
   }
   if (a.G > 1) {
-    // publish; the row's last workgroup joins the segments
-    u2v* mine = a.cand + (uint64_t)blockIdx.x * CAND_CAP;
-    if (wv == 0) {
-      if (lane == 0) {
-        G(a.part)[(uint64_t)b * a.G + g] = f2v{M, S};
-        G(mine)[0] = u2v{C, N};
-      }
-      if (TOP && lane < N) {
-        const uint64_t k = all[lane];
-        G(mine)[1 + lane] = u2v{(uint32_t)k, (uint32_t)(k >> 32)};
-      }
-      wait_stores();
+    // What the row's last workgroup reads is written and read at agent scope,
+    // past the XCDs' own caches: ordered by the wait for these stores alone.
+    // (Plain stores and a fence per workgroup, which writes the whole L2 back,
+    // took 131 us instead of 29 for 256 rows of 8 segments.)
+    uint32_t* part = a.part + (uint64_t)blockIdx.x * 4;
+    float* tmax = a.tmax + (uint64_t)b * (2 * MAX_SLOTS);
+    if (TOP)
+      for (uint32_t i = tid; i < t1 - t0; i += LT) put_agent((uint32_t*)tmax + t0 + i, __float_as_uint(s_tmax[i]));
+    if (tid == 0) {
+      put_agent(part, __float_as_uint(M));
+      put_agent(part + 1, __float_as_uint(S));
+      put_agent(part + 2, C);
     }
+    wait_stores();
     __syncthreads();
     if (tid == 0) {
-      __threadfence();
-      const uint32_t seen = atomicAdd(a.arrive + b, 1u);
-      s_last = seen == a.G - 1;
-      if (s_last) {
-        __threadfence();
-        G(a.arrive)[b] = 0;  // for the next call
-      }
+      const uint32_t last = __hip_atomic_fetch_add(a.arrive + b, 1u, __ATOMIC_RELAXED,
+                                                   __HIP_MEMORY_SCOPE_AGENT) == a.G - 1;
+      if (last) put_agent(a.arrive + b, 0u);  // for the next call
+      s_last = last;
     }
     __syncthreads();
-    if (!s_last || wv != 0) return;
-    const u2v* first = a.cand + (uint64_t)b * a.G * CAND_CAP;
+    if (!s_last) return;
+    const uint32_t* first = a.part + (uint64_t)b * a.G * 4;
     float m1 = NEG_INF, s1 = 0.0f;
-    uint32_t c1 = 0, n1 = 0;
+    uint32_t c1 = 0;
     if (lane < a.G) {
-      const f2v ms = G(a.part)[(uint64_t)b * a.G + lane];
-      const u2v cn = G(first)[(uint64_t)lane * CAND_CAP];
-      m1 = ms[0];
-      s1 = ms[1];
-      c1 = cn[0];
-      n1 = cn[1];
+      m1 = __uint_as_float(get_agent(first + 4 * lane));
+      s1 = __uint_as_float(get_agent(first + 4 * lane + 1));
+      c1 = get_agent(first + 4 * lane + 2);
     }
+    if (TOP)
+      for (uint32_t i = tid; i < a.ntiles; i += LT)
+        s_tmax[i] = __uint_as_float(get_agent((const uint32_t*)tmax + i));
     M = wave_max(m1);
     S = wave_tree_sum(m1 == NEG_INF ? 0.0f : s1 * exp_diff(m1, M));
     C = bcast63u(wave_incl_scan(c1));
-    if (TOP) {
-      // of the segments' lists, the entries not below the top_n-th largest
-      // value; entry i of the G * top_n belongs to segment i / top_n
-      constexpr int Q = TMERGE / 64;
-      uint32_t hi[Q], lo[Q];
-#pragma unroll
-      for (int i = 0; i < Q; ++i) {
-        const uint32_t at = i * 64 + lane, sg = at / a.top_n;
-        hi[i] = lo[i] = 0;
-        if (sg < a.G) {
-          const u2v k = G(first)[(uint64_t)sg * CAND_CAP + 1 + at % a.top_n];
-          const uint32_t ns = G(first)[(uint64_t)sg * CAND_CAP][1];
-          if (at % a.top_n < ns) {
-            lo[i] = k[0];
-            hi[i] = k[1];
-          }
-        }
-      }
-      const uint32_t least = nth_key<Q>(hi, a.top_n);
-      N = 0;
-#pragma unroll
-      for (int i = 0; i < Q; ++i) {
-        const bool take = hi[i] >= least && hi[i] != 0;
-        const uint64_t who = __ballot(take);
-        if (take) all[N + lanes_below(who)] = ((uint64_t)hi[i] << 32) | lo[i];
-        N += (uint32_t)__popcll(who);
-      }
-      N = keep_first<Q>(all, N, a.top_n);
-    }
+    __syncthreads();
   }
   // log p(x) = (x - M) - log S; a raw logit of -inf has none
   const float logS = __logf(S);
@@ -621,14 +564,163 @@ __global__ __launch_bounds__(LT) void logprobs_kernel(LArgs a) {
     const float y = DT & SOFTCAP ? tanh_ref(raw_x * a.sc_m1) * a.sc_cap : raw_x;
     return (y - M) - logS;
   };
-  if (lane == 0 && a.tokens) {
+  if (tid == 0 && a.tokens) {
     G(a.out_lp)[b] = chosen ? logp(lt) : __builtin_nanf("");
     if (a.out_rank) G(a.out_rank)[b] = chosen ? C : EMPTY;
   }
-  if (TOP && lane < a.top_n) {
-    const uint64_t k = lane < N ? all[lane] : 0u;
-    G(a.out_ids)[(uint64_t)b * a.top_n + lane] = k ? ~(uint32_t)k : EMPTY;
-    G(a.out_top)[(uint64_t)b * a.top_n + lane] = k ? logp(key_value(k)) : NEG_INF;
+  if (!TOP) return;
+  // The first top_n groups of tiles (a group is one tile up to 256 of them), by
+  // one wave: a lower bound of the top_n-th largest maximum, bit by bit until
+  // few more than top_n groups reach it, and those groups; where many are
+  // equal to it, the first of them.
+  const uint32_t per = (a.ntiles + 255) / 256, groups = (a.ntiles + per - 1) / per;
+  if (wv == 0) {
+    const uint32_t n = umin(a.top_n, groups), most = umin(TOP_MAX, n + 4);
+    uint32_t key[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t at = i * 64 + lane;
+      key[i] = 0;
+      for (uint32_t j = at * per; j < umin(at * per + per, a.ntiles); ++j)
+        key[i] = umax(key[i], fkey(s_tmax[j] + 0.0f));
+    }
+    auto reach = [&](uint32_t c) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m += (uint32_t)__popcll(__ballot(key[i] >= c));
+      return m;
+    };
+    uint32_t bound = wave_max_u32(umax(umax(key[0], key[1]), umax(key[2], key[3])));
+    uint32_t many = reach(bound);
+    if (many < n) {
+      bound = 0;
+      many = groups;
+#pragma unroll 1
+      for (uint32_t bit = 0x80000000u; bit && many > most; bit >>= 1) {
+        const uint32_t m = reach(bound | bit);
+        if (m >= n) {
+          bound |= bit;
+          many = m;
+        }
+      }
+    }
+    uint32_t equal = many > most ? n - reach(bound + 1) : EMPTY, at = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t eq = __ballot(key[i] == bound);
+      const bool take = key[i] && (key[i] > bound || (key[i] == bound && lanes_below(eq) < equal));
+      const uint64_t who = __ballot(take);
+      if (take) s_sel[at + lanes_below(who)] = i * 64 + lane;
+      at += (uint32_t)__popcll(who);
+      equal -= umin(equal, (uint32_t)__popcll(eq));
+    }
+    if (lane == 0) {
+      s_n[0] = at;
+      s_bound = n == a.top_n ? bound : 0u;
+    }
+  }
+  __syncthreads();
+  const uint32_t ns = s_n[0];
+  // Nothing below the bound belongs to the list (if there are top_n groups):
+  // what does not fall below is gathered by all waves.
+  const float least = s_bound > fkey(NEG_INF) ? funkey(s_bound) : NEG_INF;
+  // the selected tiles in turn, a wave each
+  auto selected = [&](uint32_t k) {
+    const uint32_t t2 = k < ns * per ? s_sel[k / per] * per + k % per : EMPTY;
+    return t2 < a.ntiles ? t2 : EMPTY;
+  };
+  auto gather = [&](const float (&x)[16], uint32_t tt) {
+    uint32_t mine = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) mine |= x[i] >= least ? 1u << i : 0u;
+    while (mine) {  // (few: the logit is read again, which keeps this code short)
+      const uint32_t e = Tile16<DT>::index(tt, (uint32_t)__builtin_ctz(mine));
+      mine &= mine - 1;
+      if (e < a.V) {
+        const uint32_t at = __hip_atomic_fetch_add((LDS uint32_t*)&s_count, 1u, __ATOMIC_RELAXED,
+                                                   __HIP_MEMORY_SCOPE_WORKGROUP);
+        if (at < LT) s_list[at] = order_key(raw_logit<DT>(row, e), e);
+      }
+    }
+  };
+  uint32_t k = wv, tt = selected(k);
+  if (tt != EMPTY) in.request(row, tt, a.V);
+  while (k < ns * per) {
+    float x[16];
+    in.values(tt == EMPTY ? a.ntiles : tt, a.V, x);
+    const uint32_t done = tt;
+    k += LWAVES;
+    tt = k < ns * per ? selected(k) : EMPTY;
+    if (tt != EMPTY) in.request(row, tt, a.V);
+    if (done != EMPTY) gather(x, done);
+  }
+  __syncthreads();
+  const uint32_t found = s_count;
+  if (found <= LT) {
+    // each thread counts the tokens before its own one
+    const uint64_t mine = tid < found ? s_list[tid] : 0u;
+    uint32_t p = 0;
+    for (uint32_t j = 0; j < found; j += 4) {  // (zeros follow the last one)
+      uint64_t o[4];
+#pragma unroll
+      for (uint32_t q = 0; q < 4; ++q) o[q] = s_list[j + q];
+#pragma unroll
+      for (uint32_t q = 0; q < 4; ++q) p += o[q] > mine ? 1u : 0u;
+    }
+    if (tid < found && p < a.top_n) {
+      G(a.out_ids)[(uint64_t)b * a.top_n + p] = ~(uint32_t)mine;
+      G(a.out_top)[(uint64_t)b * a.top_n + p] = logp(key_value(mine));
+    }
+    if (tid >= found && tid < a.top_n) {
+      G(a.out_ids)[(uint64_t)b * a.top_n + tid] = EMPTY;
+      G(a.out_top)[(uint64_t)b * a.top_n + tid] = NEG_INF;
+    }
+    return;
+  }
+  // More than that (rows of equal logits, masked rows with fewer tokens left
+  // than the list holds): by lists that keep the first top_n.
+  __syncthreads();
+  LDS uint64_t* list = (LDS uint64_t*)s_list + wv * TLIST;
+  uint32_t held = 0;
+  uint64_t bar = ((uint64_t)fkey(least) << 32) - 1;
+  for (k = wv; k < ns * per; k += LWAVES) {
+    tt = selected(k);
+    if (tt == EMPTY) continue;
+#pragma unroll 4
+    for (uint32_t i = 0; i < 16; ++i) {
+      const uint32_t e = tt * TILE + i * 64 + lane;
+      const uint64_t key = e < a.V ? order_key(raw_logit<DT>(row, e), e) : 0u;
+      const bool take = key > bar;
+      const uint64_t who = __ballot(take);
+      if (who) {
+        if (take) list[held + lanes_below(who)] = key;
+        held += (uint32_t)__popcll(who);
+        if (held > TLIST - 64) {
+          held = keep_first<TLIST / 64>(list, held, a.top_n);
+          if (held == a.top_n) bar = list[a.top_n - 1];
+        }
+      }
+    }
+  }
+  held = keep_first<TLIST / 64>(list, held, a.top_n);
+  if (lane == 0) s_n[wv] = held;
+  __syncthreads();
+  if (wv != 0) return;
+  // the waves' lists end to end (each moves down, none past its own start)
+  LDS uint64_t* all = (LDS uint64_t*)s_list;
+  uint32_t N = s_n[0];
+  for (uint32_t i = 1; i < LWAVES; ++i) {
+    const uint32_t ni = s_n[i];
+    const uint64_t x = lane < ni ? all[i * TLIST + lane] : 0u;
+    wave_sync();
+    if (lane < ni) all[N + lane] = x;
+    N += ni;
+  }
+  N = keep_first<LWAVES * TOP_MAX / 64>(all, N, a.top_n);
+  if (lane < a.top_n) {
+    const uint64_t x = lane < N ? all[lane] : 0u;
+    G(a.out_ids)[(uint64_t)b * a.top_n + lane] = x ? ~(uint32_t)x : EMPTY;
+    G(a.out_top)[(uint64_t)b * a.top_n + lane] = x ? logp(key_value(x)) : NEG_INF;
   }
 }
 
@@ -807,29 +899,38 @@ extern "C" int llmk_logprobs(llmk_sampler* s, const llmk_logprobs_args* in, void
   a.out_ids = in->out_top_ids;
   a.out_top = in->out_top_logprobs;
   a.arrive = s->ws.row_arrive;
-  a.part = s->ws.tile_part;
-  a.cand = s->ws.cand;
+  a.tmax = (float*)s->ws.tile_part;
+  a.part = (uint32_t*)s->ws.cand;
   a.ntiles = (a.V + TILE - 1) / TILE;
-  // Segments per row: 1024 workgroups, four a CU, while each wave has a tile;
-  // the segments' lists fit the last workgroup's (TMERGE) and the workspace.
-  const uint32_t pool = s->max_batch > MAX_WGS ? s->max_batch : MAX_WGS;
-  uint32_t g = (1024 + a.B - 1) / a.B;
-  const uint32_t most = (a.ntiles + LWAVES - 1) / LWAVES;
+  // The workgroup's size only matters to the last steps of a row with a top
+  // list, where one workgroup reads tiles again: the more waves the shorter
+  // they take, but the fewer rows a CU holds meanwhile.  Measured with 256,
+  // 512 and 1024 threads: 256 x 151936 f32 top 8: 35.0, 33.0, 30.9 us; 64 x
+  // 50257 f32 top 5: 14.9, 11.9, 11.5; 16 x 32000 f32: 10.8, 9.4, 10.1; 1000 x
+  // 100000 bf16 top 3: 47.2, 43.8, 47.1; 2047 x 32000 f16 top 1: 31.6, 33.4,
+  // 43.8.
+  const uint32_t lt = !in->top_n ? 256 : (a.ntiles < 40 ? (a.B <= 256 ? 512 : 256)
+                                                        : (a.B <= 256 ? 1024 : 512));
+  // Segments per row: 4096 waves, four on each SIMD, while each has a tile.
+  const uint32_t pool = s->max_batch > MAX_WGS ? s->max_batch : MAX_WGS, waves = lt / WAVE;
+  uint32_t g = (4096 / waves + a.B - 1) / a.B;
+  const uint32_t most = (a.ntiles + waves - 1) / waves;
   if (g > most) g = most;
   if (g > MAX_SEG) g = MAX_SEG;
-  if (a.top_n && g > TMERGE / a.top_n) g = TMERGE / a.top_n;
   if (a.B > s->max_batch || (uint64_t)a.B * g > pool) g = 1;
   a.tps = (a.ntiles + g - 1) / g;
   a.G = (a.ntiles + a.tps - 1) / a.tps;
   const uint64_t blocks = (uint64_t)a.B * a.G;
   if (blocks > 0x7fffffffu) return fail(LLMK_ERR_CAPACITY, "batch above 2^31 - 1");
   auto launch = [&](auto kern) {
-    hipLaunchKernelGGL(kern, dim3((uint32_t)blocks), dim3(LT), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(kern, dim3((uint32_t)blocks), dim3(lt), 0, (hipStream_t)stream, a);
   };
-#define LLMK_LOGPROBS(DT)                                     \
-  do {                                                        \
-    if (in->top_n) launch(logprobs_kernel<DT, true>);         \
-    else launch(logprobs_kernel<DT, false>);                  \
+#define LLMK_LOGPROBS(DT)                                              \
+  do {                                                                 \
+    if (!in->top_n) launch(logprobs_kernel<DT, false, 256>);           \
+    else if (lt == 256) launch(logprobs_kernel<DT, true, 256>);        \
+    else if (lt == 512) launch(logprobs_kernel<DT, true, 512>);        \
+    else launch(logprobs_kernel<DT, true, 1024>);                      \
   } while (0)
   const bool sc = in->softcap > 0.0f;
   if (in->dtype == LLMK_F32) {
