@@ -12,6 +12,7 @@
 #include <stdint.h>
 
 #include <string>
+#include <type_traits>
 
 #include "llmk_device.h"
 #include "llmk_host.h"
@@ -92,47 +93,87 @@ struct PArgs {
   uint32_t* status;
 };
 
-constexpr uint32_t PT = 256;  // threads of a workgroup
+// The softcap (DT & SOFTCAP) of a logit; a logit from memory.
+template <int DT>
+__device__ __forceinline__ float cap_f32(const PArgs& a, float x) {
+  return DT & SOFTCAP ? tanh_ref(x * a.sc_m1) * a.sc_cap : x;
+}
+template <int DT>
+__device__ __forceinline__ float raw_f32(const void* row, uint32_t e) {
+  return Elem<DT>::SZ == 4 ? G((const float*)row)[e] : cvt16<DT>(G((const uint16_t*)row)[e]);
+}
 
-// Adds the list's tokens that fall in [lo, lo + n) to their counts.
-__device__ __forceinline__ void count_tokens(LDS uint32_t* cnt, const uint32_t* tok,
-                                             const uint32_t* times, uint32_t len, uint32_t lo,
-                                             uint32_t n) {
-  auto add = [&](uint32_t t, uint32_t k) {
-    if (t - lo < n)
-      __hip_atomic_fetch_add(cnt + (t - lo), k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-  };
-  const uint32_t whole = len & ~3u;
-  for (uint32_t j = 4 * threadIdx.x; j < whole; j += 4 * PT) {
-    const u4v_list t = *(const GLB u4v_list*)G(tok + j);
-    u4v_list k = {1, 1, 1, 1};
-    if (times) k = *(const GLB u4v_list*)G(times + j);
+
+// x / T as IEEE division rounds it, for 2^-17 < T < 2^20: with r = 1 / T
+// rounded, two steps q += (x - q T) r (each residual one fused operation, so
+// exact) leave the correctly rounded quotient (Markstein: the last step does
+// if r is the rounded reciprocal of a T whose significand is not all ones and
+// q is within a unit of the quotient).  Five operations instead of a dozen.
+// Numbers that could leave the normal range on the way, zeros, infinities and
+// NaN take the division itself.
+struct Divisor {
+  float T, r;
+  bool fast;
+};
+__device__ __forceinline__ Divisor divisor(float T) {
+  const uint32_t m = __float_as_uint(T) & 0x7fffffu;
+  return {T, 1.0f / T, T > 0x1p-17f && T < 0x1p+20f && m != 0x7fffffu};
+}
+__device__ __forceinline__ void divide4(float* x, const Divisor& d) {
+  const float hi = fmaxf(fmaxf(__builtin_fabsf(x[0]), __builtin_fabsf(x[1])),
+                         fmaxf(__builtin_fabsf(x[2]), __builtin_fabsf(x[3])));
+  const float lo = fminf(fminf(__builtin_fabsf(x[0]), __builtin_fabsf(x[1])),
+                         fminf(__builtin_fabsf(x[2]), __builtin_fabsf(x[3])));
+  const float all = x[0] + x[1] + x[2] + x[3];  // NaN if one is (hi and lo leave it out)
+  if (d.fast && hi < 0x1p+100f && lo > 0x1p-90f && all == all) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) add(t[q], times && k[q] == 0 ? 1u : k[q]);
-  }
-  const uint32_t j = whole + threadIdx.x;
-  if (j < len) {
-    const uint32_t k = times ? G(times)[j] : 1u;
-    add(G(tok)[j], k ? k : 1u);
+    for (int k = 0; k < 4; ++k) {
+      float q = x[k] * d.r;
+      q = __builtin_fmaf(__builtin_fmaf(-q, d.T, x[k]), d.r, q);
+      x[k] = __builtin_fmaf(__builtin_fmaf(-q, d.T, x[k]), d.r, q);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = x[k] / d.T;
   }
 }
 
-// One workgroup per (row, segment of PT * W * CH logits).  A thread requests
-// its logits first; while they travel, the workgroup counts the history's
-// tokens of the segment in LDS, one word per logit (a segment is small enough
-// for that, and it needs no table, no hash and no limit on a history), and
-// then reads the counts back beside its logits: 4 bytes of LDS a logit, far
-// below what LDS delivers in the time of the logit's HBM traffic.  The
-// segments of a row re-read its history from L2, so they share an XCD.
+// A barrier for LDS alone: requests to memory stay on their way across it
+// (__syncthreads waits for them).
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+constexpr uint32_t TOUCHED = 2048;  // tokens listed per segment (below)
+
+// One workgroup per (row, segment of PT * N logits).  LDS holds a word per
+// logit of the segment: how often its token occurs, less one (all ones:
+// never).  A segment is small enough for a word per logit, so this needs no
+// table, no hash and no limit on a history.  A row with biases first uses the
+// words for those: each token's bias, or, where a token is listed more than
+// once, its first place in the list, from which on its biases are summed in
+// listing order, whatever order threads run in.
 //
-// Biases are added in the same way through a word of LDS per logit.  A token
-// listed more than once gets its biases summed in listing order: the first
-// entry (an LDS minimum over the list's positions) sums all of them, so the
-// result does not depend on the order in which threads run.
-template <int DT, int OT, int CH>
-__global__ __launch_bounds__(PT) void process_kernel(PArgs a) {
+// Bound by HBM without lists (512 x 128256 bf16 to bf16 47 us, 5.5 TB/s).  With
+// them by the steps before the last logit can be written: extents, tokens,
+// words, each a wait that only the CU's other three workgroups fill (with
+// histories of 1000 tokens 74 us; 256 x 151936 f32 with 2048 tokens 65 us,
+// 4.8 TB/s).  So the tokens are requested before the logits (loads come back
+// in order), barriers wait for LDS alone, and the penalties are computed where
+// the logits are, though that costs a wave an operation for each of its
+// logits as soon as one of the 64 neighbours has a count: a list of the touched
+// tokens, penalised by a thread each from memory, took 71 us instead of 65.
+// TOUCHED_ONLY, for calls in place that change no other logit (no softcap, bias,
+// mask or temperature), has such a list, and reads and writes nothing else.
+// Fewer, longer workgroups that run over several segments with the next one's
+// logits on their way took 90 us: fewer of them fit a CU.  The segments of a
+// row re-read its lists from L2, so they share an XCD.
+template <int DT, int OT, uint32_t PT, bool TOUCHED_ONLY>
+__global__ __launch_bounds__(PT, 8) void process_kernel(PArgs a) {
   extern __shared__ uint32_t psm[];
-  constexpr uint32_t W = Elem<DT>::W, SEG = PT * W * CH;
+  __shared__ uint16_t s_list[TOUCHED_ONLY ? TOUCHED : 1];
+  __shared__ uint32_t s_listed, s_twice;
+  constexpr uint32_t W = Elem<DT>::W, N = PT == 512 ? 16 : 8, CH = N / W, SEG = PT * N;
   const uint32_t tid = threadIdx.x;
   uint32_t b, g;
   if ((a.B & 7u) == 0) {  // blocks go round the 8 XCDs: a row's segments on one
@@ -147,135 +188,198 @@ __global__ __launch_bounds__(PT) void process_kernel(PArgs a) {
   const char* row = (const char*)a.in + (uint64_t)b * a.in_stride * Elem<DT>::SZ;
   char* orow = (char*)a.out + (uint64_t)b * a.out_stride * Elem<OT>::SZ;
 
-  u4v r[CH];
-#pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    const uint32_t e = lo + (c * PT + tid) * W;
-    r[c] = u4v{0, 0, 0, 0};
-    if (e < a.V) r[c] = load_pack<DT>(row, e, a.V);
-  }
-
   const uint32_t q = a.row_seq ? G(a.row_seq)[b] : b;
-  bool bad = a.row_seq && q >= a.sequences;
-  const uint32_t qs = bad ? 0u : q;
   int32_t mi = -1;
-  if (a.mask) {
-    mi = a.mask_index ? G(a.mask_index)[b] : (int32_t)b;
-    if (mi >= 0 && (uint32_t)mi >= a.mask_rows) bad = true;
-  }
+  if (a.mask) mi = a.mask_index ? G(a.mask_index)[b] : (int32_t)b;
+  const uint32_t x0 = *G(row_or(a.xbeg, b, &kZeroU)), xc = *G(row_or(a.xcnt, b, &kZeroU));
+  bool bad = (a.row_seq && q >= a.sequences) || (mi >= 0 && (uint32_t)mi >= a.mask_rows);
+  const uint32_t qs = a.row_seq && q >= a.sequences ? 0u : q;
   RowP P;
   P.T = *G(row_or(a.T, qs, &kOneF));
   P.rp = *G(row_or(a.rp, qs, &kOneF));
   P.pp = *G((const float*)row_or(a.pp, qs, &kZeroU));
   P.fp = *G((const float*)row_or(a.fp, qs, &kZeroU));
+  const uint32_t h0 = *G(row_or(a.hoff, qs, &kZeroU));
+  const uint32_t hl = *G(row_or(a.hlen, qs, &kZeroU));
+  const uint32_t he = *G(row_or(a.hlen ? nullptr : a.hoff, qs + 1, &kZeroU));
+  const uint32_t j0 = *G(row_or(a.boff, qs, &kZeroU)), j1 = *G(row_or(a.boff, qs + 1, &kZeroU));
   if (!finitef(P.T) || !finitef(P.rp) || !finitef(P.pp) || !finitef(P.fp)) bad = true;
   if (bad) {  // the whole workgroup agrees
     for (uint32_t e = lo + tid; e < lo + n; e += PT) store_one<OT>(orow, e, __builtin_nanf(""));
     if (g == 0 && tid == 0) atomicOr(a.status, LLMK_STATUS_INVALID_PARAMS);
     return;
   }
+
+  // the lists: the first tokens of each thread
+  const bool pen = P.rp != 1.0f || P.pp != 0.0f || P.fp != 0.0f;
+  const uint32_t h1 = a.hlen ? h0 + hl : he;
+  const uint32_t hn = pen && h1 > h0 ? h1 - h0 : 0u, xn = pen ? xc : 0u;
+  const uint32_t nb = j1 > j0 ? j1 - j0 : 0u, whole = hn & ~3u;
+  const uint32_t *ht = a.htok + h0, *hc = a.hcnt ? a.hcnt + h0 : nullptr;
+  const uint32_t *xt = a.xtok + x0, *bt = a.btok + j0;
+  const float* bv = a.bval + j0;
+  u4v_list ht0 = {EMPTY, EMPTY, EMPTY, EMPTY}, hc0 = {1, 1, 1, 1};
+  uint32_t ht1 = EMPTY, hc1 = 1, xt0 = EMPTY, bt0 = EMPTY, bv0 = 0;
+  if (4 * tid < whole) {
+    ht0 = *(const GLB u4v_list*)G(ht + 4 * tid);
+    if (hc) hc0 = *(const GLB u4v_list*)G(hc + 4 * tid);
+  }
+  if (whole + tid < hn) {
+    ht1 = G(ht)[whole + tid];
+    if (hc) hc1 = G(hc)[whole + tid];
+  }
+  if (tid < xn) xt0 = G(xt)[tid];
+  if (tid < nb) {
+    bt0 = G(bt)[tid];
+    bv0 = G((const uint32_t*)bv)[tid];
+  }
+  // the mask's words and the logits
   const uint32_t* mrow =
       a.mask && mi >= 0 ? a.mask + (uint64_t)(uint32_t)mi * a.mask_words : nullptr;
   uint32_t mw[CH];
+  if (mrow) {
 #pragma unroll
-  for (int c = 0; c < CH; ++c) {
-    const uint32_t e = lo + (c * PT + tid) * W;
-    mw[c] = 0xffffffffu;
-    if (mrow && e < a.V) mw[c] = G(mrow)[e >> 5] >> (e & 31u);  // W divides 32
+    for (uint32_t c = 0; c < CH; ++c) {
+      const uint32_t e = lo + (c * PT + tid) * W;
+      mw[c] = e < a.V ? G(mrow)[e >> 5] >> (e & 31u) : 0u;  // W divides 32
+    }
   }
+  u4v r[CH];
+  auto request = [&]() {
+#pragma unroll
+    for (uint32_t c = 0; c < CH; ++c) {
+      const uint32_t e = lo + (c * PT + tid) * W;
+      r[c] = u4v{0, 0, 0, 0};
+      if (e < a.V) r[c] = load_pack<DT>(row, e, a.V);
+    }
+  };
+  if (!TOUCHED_ONLY) request();
 
   LDS uint32_t* cnt = (LDS uint32_t*)psm;
-  LDS float* bsum = (LDS float*)psm + SEG;  // present if a.boff
-  bool bias = false;
-  if (a.boff) {
-    const uint32_t j0 = G(a.boff)[qs], j1 = G(a.boff)[qs + 1];
-    const uint32_t nb = j1 > j0 ? j1 - j0 : 0u;
-    bias = nb > 0;
-    if (bias) {
-      const uint32_t* bt = a.btok + j0;
-      for (uint32_t i = tid; i < SEG; i += PT) {
-        cnt[i] = EMPTY;
-        bsum[i] = 0.0f;
-      }
-      __syncthreads();
+  LDS uint16_t* list = (LDS uint16_t*)s_list;
+  auto clear = [&]() {
+    for (uint32_t i = tid; i < SEG / 4; i += PT)
+      *(LDS u4v*)(cnt + 4 * i) = u4v{EMPTY, EMPTY, EMPTY, EMPTY};
+  };
+  float add[N];  // biases of the thread's logits
+  if (hn | xn | nb) {
+    clear();
+    if (tid == 0) s_listed = s_twice = 0;
+    lds_barrier();
+  }
+  if (nb && !TOUCHED_ONLY) {
+    for (uint32_t j = tid; j < nb; j += PT) {
+      const uint32_t t = (j == tid ? bt0 : G(bt)[j]) - lo;
+      const uint32_t v = j == tid ? bv0 : __float_as_uint(G(bv)[j]);
+      if (t < n && __hip_atomic_exchange(cnt + t, v == EMPTY ? 0x7fc00000u : v, __ATOMIC_RELAXED,
+                                         __HIP_MEMORY_SCOPE_WORKGROUP) != EMPTY)
+        s_twice = 1;
+    }
+    lds_barrier();
+    const bool twice = s_twice != 0;
+    if (twice) {  // the first place of each token instead of its bias
+      clear();
+      lds_barrier();
       for (uint32_t j = tid; j < nb; j += PT) {
-        const uint32_t t = G(bt)[j] - lo;
+        const uint32_t t = (j == tid ? bt0 : G(bt)[j]) - lo;
         if (t < n)
           __hip_atomic_fetch_min(cnt + t, j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
       }
-      __syncthreads();
-      for (uint32_t j = tid; j < nb; j += PT) {  // later entries mark the first one's word
-        const uint32_t t = G(bt)[j] - lo;
-        if (t < n && (cnt[t] & 0x7fffffffu) != j)
-          __hip_atomic_fetch_or(cnt + t, 0x80000000u, __ATOMIC_RELAXED,
-                                __HIP_MEMORY_SCOPE_WORKGROUP);
-      }
-      __syncthreads();
-      for (uint32_t j = tid; j < nb; j += PT) {
-        const uint32_t tok = G(bt)[j], t = tok - lo;
-        if (t < n) {
-          const uint32_t w = cnt[t];
-          if ((w & 0x7fffffffu) == j) {
-            float v = G(a.bval)[j0 + j];
-            if (w >> 31)
-              for (uint32_t k = j + 1; k < nb; ++k)
-                if (G(bt)[k] == tok) v += G(a.bval)[j0 + k];
-            bsum[t] = v;
-          }
-        }
-      }
-      __syncthreads();
+      lds_barrier();
     }
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) {
+      const uint32_t t = ((i / W) * PT + tid) * W + i % W, w = cnt[t];
+      add[i] = w == EMPTY ? 0.0f : __uint_as_float(w);
+      if (w == EMPTY) continue;
+      cnt[t] = EMPTY;  // for the counts
+      if (twice) {
+        add[i] = G(bv)[w];
+        for (uint32_t k = w + 1; k < nb; ++k)
+          if (G(bt)[k] == lo + t) add[i] += G(bv)[k];
+      }
+    }
+    lds_barrier();
   }
-  const bool pen = P.rp != 1.0f || P.pp != 0.0f || P.fp != 0.0f;
-  bool have = false;
-  if (pen && (a.hoff || a.xbeg)) {
-    const uint32_t h0 = a.hoff ? G(a.hoff)[qs] : 0u;
-    const uint32_t h1 = a.hoff ? (a.hlen ? h0 + G(a.hlen)[qs] : G(a.hoff)[qs + 1]) : 0u;
-    const uint32_t hn = h1 > h0 ? h1 - h0 : 0u, xn = a.xbeg ? G(a.xcnt)[b] : 0u;
-    have = hn > 0 || xn > 0;
-    if (have) {
-      for (uint32_t i = tid; i < SEG / 4; i += PT) *(LDS u4v*)(cnt + 4 * i) = u4v{0, 0, 0, 0};
-      __syncthreads();
-      if (hn) count_tokens(cnt, a.htok + h0, a.hcnt ? a.hcnt + h0 : nullptr, hn, lo, n);
-      if (xn) count_tokens(cnt, a.xtok + G(a.xbeg)[b], nullptr, xn, lo, n);
-      __syncthreads();
+  if (hn | xn) {
+    // the atomics of several tokens together, then what they found
+    auto count = [&](auto tok, auto times, auto how_many) {
+      constexpr int K = decltype(how_many)::value;
+      uint32_t was[K];
+#pragma unroll
+      for (int i = 0; i < K; ++i) {
+        const uint32_t t = tok(i) - lo, k = times(i);
+        was[i] = 0;
+        if (t < n)
+          was[i] = __hip_atomic_fetch_add(cnt + t, k ? k : 1u, __ATOMIC_RELAXED,
+                                          __HIP_MEMORY_SCOPE_WORKGROUP);
+      }
+#pragma unroll
+      for (int i = 0; i < K; ++i) {
+        if (!TOUCHED_ONLY || was[i] != EMPTY) continue;
+        const uint32_t at = __hip_atomic_fetch_add((LDS uint32_t*)&s_listed, 1u, __ATOMIC_RELAXED,
+                                                   __HIP_MEMORY_SCOPE_WORKGROUP);
+        if (at < TOUCHED) list[at] = (uint16_t)(tok(i) - lo);
+      }
+    };
+    count([&](int i) { return i < 4 ? ht0[i & 3] : i == 4 ? ht1 : xt0; },
+          [&](int i) { return i < 4 ? hc0[i & 3] : i == 4 ? hc1 : 1u; },
+          std::integral_constant<int, 6>());
+    for (uint32_t j = 4 * (PT + tid); j < whole; j += 4 * PT) {
+      const u4v_list t = *(const GLB u4v_list*)G(ht + j);
+      u4v_list k = {1, 1, 1, 1};
+      if (hc) k = *(const GLB u4v_list*)G(hc + j);
+      count([&](int i) { return t[i]; }, [&](int i) { return k[i]; },
+            std::integral_constant<int, 4>());
     }
+    for (uint32_t j = PT + tid; j < xn; j += PT) {
+      const uint32_t t = G(xt)[j];
+      count([&](int) { return t; }, [](int) { return 1u; }, std::integral_constant<int, 1>());
+    }
+    lds_barrier();
+  }
+  if (TOUCHED_ONLY) {  // the touched logits alone, by the list or, if it is full, by the words
+    const uint32_t listed = hn | xn ? s_listed : 0u, m = listed > TOUCHED ? n : listed;
+    for (uint32_t i = tid; i < m; i += PT) {
+      const uint32_t t = listed > TOUCHED ? i : list[i], c = cnt[t] + 1u;
+      if (c) store_one<OT>(orow, lo + t, penalize(raw_f32<DT>(row, lo + t), P, c));
+    }
+    return;
   }
   const bool divide = P.T != 1.0f && P.T > 1e-5f;
+  const Divisor D = divisor(P.T);
 
 #pragma unroll
-  for (int c = 0; c < CH; ++c) {
+  for (uint32_t c = 0; c < CH; ++c) {
     const uint32_t at = (c * PT + tid) * W, e = lo + at;
     if (e >= a.V) break;
     float x[W];
 #pragma unroll
-    for (uint32_t k = 0; k < W; ++k) {
-      x[k] = unpack<DT>(r[c], k);
-      if (DT & SOFTCAP) x[k] = tanh_ref(x[k] * a.sc_m1) * a.sc_cap;
-    }
-    if (bias) {
+    for (uint32_t k = 0; k < W; ++k) x[k] = cap_f32<DT>(a, unpack<DT>(r[c], k));
+    if (nb) {
 #pragma unroll
       for (uint32_t k = 0; k < W; ++k) {
-        const float v = bsum[at + k];
+        const float v = add[c * W + k];
         if (v != 0.0f) x[k] += v;  // (a logit of -0 without a bias stays -0)
       }
     }
-    if (have) {
+    if (hn | xn) {
 #pragma unroll
       for (uint32_t h = 0; h < W; h += 4) {
         const u4v m = *(LDS u4v*)(cnt + at + h);
-        if (m[0] | m[1] | m[2] | m[3]) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (m[k]) x[h + k] = penalize(x[h + k], P, m[k]);
-        }
+        for (uint32_t k = 0; k < 4; ++k)
+          if (m[k] != EMPTY) x[h + k] = penalize(x[h + k], P, m[k] + 1u);
       }
     }
+    if (divide) {
 #pragma unroll
-    for (uint32_t k = 0; k < W; ++k) {
-      if (!((mw[c] >> k) & 1u)) x[k] = NEG_INF;
-      if (divide) x[k] = x[k] / P.T;
+      for (uint32_t h = 0; h < W; h += 4) divide4(x + h, D);
+    }
+    if (mrow) {
+#pragma unroll
+      for (uint32_t k = 0; k < W; ++k)
+        if (!((mw[c] >> k) & 1u)) x[k] = NEG_INF;
     }
     if (e + W <= a.V) {
       if (OT == LLMK_F32) {
@@ -845,17 +949,21 @@ extern "C" int llmk_process_logits(llmk_sampler* s, const llmk_process_logits_ar
   a.status = s->ws.status;
   const bool sc = in->softcap > 0.0f;
   const bool counts = in->hist_offsets || in->extra_begin;
-  const size_t lds = in->bias_offsets ? 8 * (size_t)seg : (counts ? 4 * (size_t)seg : 0);
+  const size_t lds = counts || in->bias_offsets ? 4 * (size_t)seg : 0;
+  const bool touched_only = in->out == in->logits && !sc && !in->temperature && !in->allow_mask &&
+                            !in->bias_offsets;
   auto launch = [&](auto kern) {
-    hipLaunchKernelGGL(kern, dim3((uint32_t)blocks), dim3(PT), lds, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(kern, dim3((uint32_t)blocks), dim3(large ? 512 : 256), lds,
+                       (hipStream_t)stream, a);
   };
 #define LLMK_PROCESS(DT, OT)                                                   \
   do {                                                                         \
-    constexpr int C = (DT) == LLMK_F32 ? 8 : 4;                                \
-    if (sc && large) launch(process_kernel<(DT) | SOFTCAP, OT, C>);            \
-    else if (sc) launch(process_kernel<(DT) | SOFTCAP, OT, C / 4>);            \
-    else if (large) launch(process_kernel<DT, OT, C>);                         \
-    else launch(process_kernel<DT, OT, C / 4>);                                \
+    if (touched_only && large) launch(process_kernel<DT, DT, 512, true>);      \
+    else if (touched_only) launch(process_kernel<DT, DT, 256, true>);          \
+    else if (sc && large) launch(process_kernel<(DT) | SOFTCAP, OT, 512, false>); \
+    else if (sc) launch(process_kernel<(DT) | SOFTCAP, OT, 256, false>);       \
+    else if (large) launch(process_kernel<DT, OT, 512, false>);                \
+    else launch(process_kernel<DT, OT, 256, false>);                           \
   } while (0)
   if (in->dtype == LLMK_F32) LLMK_PROCESS(LLMK_F32, LLMK_F32);
   else if (in->dtype == LLMK_BF16 && in->out_dtype == LLMK_F32) LLMK_PROCESS(LLMK_BF16, LLMK_F32);

@@ -566,3 +566,31 @@ def test_tensors_of_another_device_are_refused(sampler):
     with pytest.raises(llmk.SamplerError, match="rows, the logits have 2"):
         sampler.process_logits(llmk.LogitsBatch(logits=torch.zeros(2, 8, device="cuda:0"),
                                                 temperature=dev([1.0], torch.float32)))
+
+
+@pytest.mark.parametrize("T", [0.7, 1.2, 0.0313, 1.9999999, 3.0, 2e-5, 4.9e5, 1e7])
+def test_division_by_the_temperature_is_the_division(sampler, T):
+    """Bit for bit IEEE's quotient, from the smallest numbers to the largest:
+    every exponent, random significands, zeros of both signs, infinities."""
+    g = torch.Generator(device="cuda:0")
+    g.manual_seed(int(T * 1000))
+    n = 1 << 20
+    bits = torch.randint(-2**31, 2**31 - 1, (n,), generator=g, device="cuda:0").int()
+    x = bits.view(torch.float32)
+    x = torch.where(torch.isnan(x), torch.randn(n, generator=g, device="cuda:0"), x)
+    x[:n // 2] = torch.randn(n // 2, generator=g, device="cuda:0") * 8
+    x[5], x[9], x[77], x[81] = 0.0, -0.0, float("inf"), float("-inf")
+    x = x.view(4, n // 4)
+    t = torch.full((4,), T, device="cuda:0")
+    got = sampler.process_logits(llmk.LogitsBatch(logits=x, temperature=t))
+    assert torch.equal(got.view(torch.int32), (x / t[:, None]).view(torch.int32))
+
+
+@pytest.mark.parametrize("inplace", [False, True])
+def test_process_a_segment_with_thousands_of_history_tokens(sampler, inplace):
+    """Nearly every token of the row is in the history, some many times, with
+    biases: more than a segment lists."""
+    case = Case(np.random.default_rng(31), 3, 20000, hist=60000, bias=5000, T=not inplace, twice=True)
+    check_process(sampler, case, "f32", inplace=inplace)
+    case = Case(np.random.default_rng(32), 80, 9000, hist=30000, T=not inplace)
+    check_process(sampler, case, "bf16", "same", inplace=inplace)
