@@ -16,6 +16,7 @@
 
 #include "llmk_device.h"
 #include "llmk_host.h"
+#include "llmk_sync.h"
 
 namespace llmk {
 
@@ -158,12 +159,6 @@ __device__ __forceinline__ void divide4(float* x, const Divisor& d) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) x[k] = x[k] / d.T;
   }
-}
-
-// A barrier for LDS alone: requests to memory stay on their way across it
-// (__syncthreads waits for them).
-__device__ __forceinline__ void lds_barrier() {
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 constexpr uint32_t TOUCHED = 2048;  // tokens listed per segment (below)
@@ -494,14 +489,6 @@ __device__ __forceinline__ float raw_logit(const void* row, uint32_t e) {
   return x == x ? x : NEG_INF;
 }
 
-// Words passed between workgroups, at agent scope.
-__device__ __forceinline__ void put_agent(uint32_t* p, uint32_t v) {
-  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ uint32_t get_agent(const uint32_t* p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
 constexpr float kLog2e = 0x1.715476p+0f;
 __device__ __forceinline__ float exp_diff(float x, float m) {  // e^(x - m), x <= m
   return __builtin_amdgcn_exp2f((x - m) * kLog2e);
@@ -640,10 +627,7 @@ __global__ __launch_bounds__(LT, 8) void logprobs_kernel(LArgs a) {
     C += s_c[i];
   }
   if (a.G > 1) {
-    // What the row's last workgroup reads is written and read at agent scope,
-    // past the XCDs' own caches: ordered by the wait for these stores alone.
-    // (Plain stores and a fence per workgroup, which writes the whole L2 back,
-    // took 131 us instead of 29 for 256 rows of 8 segments.)
+    // what the row's last workgroup reads
     uint32_t* part = a.part + (uint64_t)blockIdx.x * 4;
     float* tmax = a.tmax + (uint64_t)b * (2 * MAX_SLOTS);
     if (TOP)

@@ -64,7 +64,8 @@ class Pair:
                                self.bytes_of(p.contents[held], i, t.shape[1]))
         # nothing is left over from one call to the next
         N, work = c.num_pages, c._work
-        moves = 2 + 2 * max(c.rows, N // 2 + 1)
+        moves = 4 + 2 * max(c.rows, N // 2 + 1)
+        assert not work[2:4].any()
         assert not work[moves:moves + 2 * N].any()
 
     def update(self, new=None, parents=None):
