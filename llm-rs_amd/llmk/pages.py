@@ -16,7 +16,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from .sampler import _I32, HipSampler, SamplerError, _flat, _on_device, _ptr
+from .sampler import _I32, HipSampler, SamplerError, _flat, _on_device, _ptr, _raw_stream
 
 
 class PagePools:
@@ -62,7 +62,7 @@ class PageCache:
             if self.pools.num_pages != num_pages:
                 raise SamplerError(_lib.LLMK_ERR_INVALID_ARGUMENT,
                                    f"pools of {self.pools.num_pages} pages, num_pages {num_pages}")
-            sampler._same_device(self.pools.addresses.device)
+            sampler._same_device(self.pools.addresses)
         if max_pages <= 0 or page_tokens <= 0:
             raise SamplerError(_lib.LLMK_ERR_INVALID_ARGUMENT,
                                "max_pages and page_tokens must be > 0")
@@ -87,10 +87,8 @@ class PageCache:
         if rc != 0:
             raise SamplerError(rc, _lib.last_error())
 
-    def _call(self, fn: str, *ptrs, stream: Optional[torch.cuda.Stream]) -> None:
-        st = stream if stream is not None else torch.cuda.current_stream(self.state.device)
-        self._check(getattr(self._lib, fn)(self.sampler._h, ctypes.byref(self._args), *ptrs,
-                                           ctypes.c_void_p(st.cuda_stream)))
+    def _stream(self, stream: Optional[torch.cuda.Stream]) -> int:
+        return _raw_stream(self.sampler.device, stream)
 
     def load(self, table: torch.Tensor, lengths: torch.Tensor) -> None:
         """The rows of a cache kept elsewhere (a checkpoint, another process):
@@ -121,14 +119,18 @@ class PageCache:
         and grow to new_lengths[r] (int32 [rows], negative: nothing asked of the
         row).  Returns int32 [rows]: 1, or 0 where a row did not get what it
         asked for (too few pages, or an invalid request)."""
-        _on_device(self.state.device, new_lengths=new_lengths, parents=parents)
         for name, t in (("new_lengths", new_lengths), ("parents", parents)):
+            if t is None:
+                continue
+            if t.get_device() != self.sampler.device:
+                _on_device(self.state.device, **{name: t})
             _flat(name, t, _I32)
-            if t is not None and t.numel() != self.rows:
+            if t.numel() != self.rows:
                 raise SamplerError(_lib.LLMK_ERR_INVALID_ARGUMENT, f"{name} needs an entry per row")
         granted = torch.empty(self.rows, dtype=torch.int32, device=self.state.device)
-        self._call("llmk_pages_update", _ptr(parents), _ptr(new_lengths), _ptr(granted),
-                   stream=stream)
+        self._check(self._lib.llmk_pages_update(
+            self.sampler._h, ctypes.byref(self._args), _ptr(parents), _ptr(new_lengths),
+            granted.data_ptr(), self._stream(stream)))
         if stream is not None:
             granted.record_stream(stream)
         return granted
@@ -137,7 +139,8 @@ class PageCache:
         """llmk_pages_compact: the pages in use move to the front.  Returns
         int32 [num_pages]: where each page's contents are now."""
         out = torch.empty(self.num_pages, dtype=torch.int32, device=self.state.device)
-        self._call("llmk_pages_compact", _ptr(out), stream=stream)
+        self._check(self._lib.llmk_pages_compact(self.sampler._h, ctypes.byref(self._args),
+                                                 out.data_ptr(), self._stream(stream)))
         if stream is not None:
             out.record_stream(stream)
         return out

@@ -182,52 +182,76 @@ def _entries(name: str, t: Optional[torch.Tensor], n: int) -> None:
                            f"{name} has {t.numel()} entries, needs {n}")
 
 
+# The arrays of a LogitsBatch, their element types, and how many entries they
+# need: "seq" one per sequence, "row" one per row.
+_PROCESS_ARRAYS = (
+    ("row_seq", _U32, "row"), ("temperature", _F32, "seq"), ("repetition_penalty", _F32, "seq"),
+    ("presence_penalty", _F32, "seq"), ("frequency_penalty", _F32, "seq"),
+    ("hist_offsets", _U32, ""), ("hist_tokens", _U32, ""), ("hist_lengths", _U32, "seq"),
+    ("hist_counts", _U32, ""), ("extra_begin", _U32, "row"), ("extra_count", _U32, "row"),
+    ("extra_tokens", _U32, ""), ("bias_offsets", _U32, ""), ("bias_tokens", _U32, ""),
+    ("bias_values", _F32, ""), ("allow_mask", _U32, ""), ("mask_index", _I32, "row"))
+
+
 def _process_args(lb: LogitsBatch, out: torch.Tensor) -> "_lib.ProcessLogitsArgs":
     """llmk_process_logits_args for lb, after checking every tensor's device,
     element type, layout and length."""
     lg = lb.logits
     a = _lib.ProcessLogitsArgs()
-    a.dtype = _logits_rows("logits", lg)
-    a.out_dtype = _logits_rows("out", out)
-    V, B = _vocab(lg, lb.vocab), lg.shape[0]
+    a.dtype, a.out_dtype = _logits_rows("logits", lg), _logits_rows("out", out)
+    B, dev = lg.shape[0], lg.get_device()
+    V = _vocab(lg, lb.vocab)
     if out.shape[0] != B or out.shape[1] < V:
         raise SamplerError(_lib.LLMK_ERR_INVALID_ARGUMENT, "out must be [batch, >= vocab]")
-    floats = ("temperature", "repetition_penalty", "presence_penalty", "frequency_penalty")
-    ints = ("row_seq", "hist_offsets", "hist_tokens", "hist_lengths", "hist_counts", "extra_begin",
-            "extra_count", "extra_tokens", "bias_offsets", "bias_tokens", "mask_index")
-    fields = {n: getattr(lb, n) for n in floats + ints + ("bias_values", "allow_mask")}
-    _on_device(lg.device, out=out, **fields)
-    for n in floats + ("bias_values",):
-        _flat(n, fields[n], _F32)
-    for n in ints + ("allow_mask",):
-        _flat(n, fields[n], _U32 if n != "mask_index" else _I32)
-    # the sequences: as many as every array that is per sequence has entries for
-    per_seq = [fields[n].numel() for n in floats + ("hist_lengths",) if fields[n] is not None]
+    if dev < 0 or out.get_device() != dev:
+        _on_device(lg.device, out=out)
+    seqs = 2**31 - 1  # as many as every array that is per sequence has entries for
+    for name, dtypes, need in _PROCESS_ARRAYS:
+        t = getattr(lb, name)
+        if t is None:
+            continue
+        if t.get_device() != dev:
+            _on_device(lg.device, **{name: t})
+        if t.dtype not in dtypes or not t.is_contiguous():
+            _flat(name, t, dtypes)
+        if need == "seq":
+            seqs = min(seqs, t.numel())
+        elif need:
+            _entries(name, t, B)
+        # (an empty array, of histories that hold nothing, is there all the same:
+        # it gets an address, which nothing reads)
+        setattr(a, name, t.data_ptr() or lg.data_ptr())
     if lb.hist_offsets is not None:
-        per_seq.append(lb.hist_offsets.numel() - (0 if lb.hist_lengths is not None else 1))
+        seqs = min(seqs, lb.hist_offsets.numel() - (0 if lb.hist_lengths is not None else 1))
+        if lb.hist_counts is not None and lb.hist_tokens is not None:
+            _entries("hist_counts", lb.hist_counts, lb.hist_tokens.numel())
     if lb.bias_offsets is not None:
-        per_seq.append(lb.bias_offsets.numel() - 1)
-    seqs = max(0, min(per_seq)) if per_seq else (B if lb.row_seq is None else 2**31 - 1)
+        seqs = min(seqs, lb.bias_offsets.numel() - 1)
+        if lb.bias_tokens is not None and lb.bias_values is not None:
+            _entries("bias_values", lb.bias_values, lb.bias_tokens.numel())
     if lb.row_seq is None and seqs < B:
         raise SamplerError(_lib.LLMK_ERR_INVALID_ARGUMENT,
                            f"per-row arrays for {seqs} rows, the logits have {B}")
-    for n in ("row_seq", "extra_begin", "extra_count", "mask_index"):
-        _entries(n, fields[n], B)
-    if lb.hist_counts is not None and lb.hist_tokens is not None:
-        _entries("hist_counts", lb.hist_counts, lb.hist_tokens.numel())
-    if lb.bias_tokens is not None and lb.bias_values is not None:
-        _entries("bias_values", lb.bias_values, lb.bias_tokens.numel())
-    if lb.allow_mask is not None and lb.allow_mask.dim() != 2:
-        raise SamplerError(_lib.LLMK_ERR_INVALID_ARGUMENT, "allow_mask must be [rows, words]")
+    if lb.allow_mask is not None:
+        if lb.allow_mask.dim() != 2:
+            raise SamplerError(_lib.LLMK_ERR_INVALID_ARGUMENT, "allow_mask must be [rows, words]")
+        a.mask_rows, a.mask_words_per_row = lb.allow_mask.shape
     a.logits, a.batch, a.vocab, a.row_stride = lg.data_ptr(), B, V, _row_stride(lg)
     a.out, a.out_stride = out.data_ptr(), _row_stride(out)
-    a.softcap = float(lb.softcap or 0.0)
-    a.sequences = seqs
-    for n, t in fields.items():
-        setattr(a, n, _ptr(t))
-    if lb.allow_mask is not None:
-        a.mask_rows, a.mask_words_per_row = lb.allow_mask.shape
+    a.softcap, a.sequences = lb.softcap or 0.0, max(0, seqs)
     return a
+
+
+# The current stream's handle without a Stream object around it (1 us less of
+# a call's 9), where torch has it.
+_current_raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _raw_stream(device: int, stream: Optional[torch.cuda.Stream]) -> int:
+    """The hipStream_t of a call: `stream`, or the device's current one."""
+    if stream is not None:
+        return stream.cuda_stream
+    return _current_raw(device) if _current_raw else torch.cuda.current_stream(device).cuda_stream
 
 
 def _batch_args(db: DeviceBatch, out_tokens: torch.Tensor,
@@ -549,26 +573,30 @@ class HipSampler:
         return tok, acc
 
     # ---- operators on logits ----------------------------------------------
-    def _same_device(self, dev: torch.device) -> None:
-        if dev.type != "cuda" or dev.index != self.device:
+    def _same_device(self, t: torch.Tensor) -> None:
+        if t.get_device() != self.device:
             raise SamplerError(_lib.LLMK_ERR_INVALID_ARGUMENT,
-                               f"tensors on {dev}, the sampler on cuda:{self.device}")
+                               f"tensors on {t.device}, the sampler on cuda:{self.device}")
 
     def process_logits(self, lb: LogitsBatch, out: Optional[torch.Tensor] = None,
                        stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
         """llmk_process_logits: softcap, logit bias, penalties, allow-mask and
         temperature of every row, into `out` ([B, >= V], float32 or the logits'
         dtype; lb.logits itself: in place), by default a new float32 tensor."""
-        if out is None:
+        new = out is None
+        if new:
             _logits_rows("logits", lb.logits)
             out = torch.empty(lb.logits.shape[0], _vocab(lb.logits, lb.vocab), dtype=torch.float32,
                               device=lb.logits.device)
         a = _process_args(lb, out)
-        self._same_device(lb.logits.device)
-        rc = self._lib.llmk_process_logits(
-            self._h, ctypes.byref(a), ctypes.c_void_p(self._stream(lb.logits, stream).cuda_stream))
+        self._same_device(lb.logits)
+        if a.batch == 0:
+            return out
+        rc = self._lib.llmk_process_logits(self._h, ctypes.byref(a), _raw_stream(self.device, stream))
         if rc != 0:
             raise SamplerError(rc, _lib.last_error())
+        if new and stream is not None:
+            out.record_stream(stream)
         return out
 
     def logprobs(self, logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
@@ -578,46 +606,53 @@ class HipSampler:
         the row's top_n likeliest tokens (ties: the lower id first)."""
         a = _lib.LogprobsArgs()
         a.dtype = _logits_rows("logits", logits)
-        _on_device(logits.device, tokens=tokens)
-        _flat("tokens", tokens, _U32)
-        self._same_device(logits.device)
+        self._same_device(logits)
         B, dev = logits.shape[0], logits.device
-        _entries("tokens", tokens, B)
-        if not 0 <= int(top_n) <= 32:
+        if not 0 <= top_n <= 32:
             raise SamplerError(_lib.LLMK_ERR_CAPACITY, "top_n outside 0 .. 32")
+        a.logits, a.batch, a.vocab = logits.data_ptr(), B, _vocab(logits, vocab)
+        a.row_stride, a.softcap = _row_stride(logits), softcap or 0.0
         r = Logprobs()
         if tokens is not None:
+            if tokens.get_device() != self.device:
+                _on_device(dev, tokens=tokens)
+            _flat("tokens", tokens, _U32)
+            _entries("tokens", tokens, B)
             r.logprobs = torch.empty(B, dtype=torch.float32, device=dev)
             r.ranks = torch.empty(B, dtype=torch.int32, device=dev)
+            a.tokens, a.out_logprobs = tokens.data_ptr(), r.logprobs.data_ptr()
+            a.out_ranks = r.ranks.data_ptr()
         if top_n:
             r.top_ids = torch.empty(B, top_n, dtype=torch.int32, device=dev)
             r.top_logprobs = torch.empty(B, top_n, dtype=torch.float32, device=dev)
-        a.logits, a.batch, a.vocab = logits.data_ptr(), B, _vocab(logits, vocab)
-        a.row_stride, a.softcap = _row_stride(logits), float(softcap or 0.0)
-        a.tokens, a.out_logprobs, a.out_ranks = _ptr(tokens), _ptr(r.logprobs), _ptr(r.ranks)
-        a.top_n, a.out_top_ids, a.out_top_logprobs = top_n, _ptr(r.top_ids), _ptr(r.top_logprobs)
-        st = self._stream(logits, stream)
-        rc = self._lib.llmk_logprobs(self._h, ctypes.byref(a), ctypes.c_void_p(st.cuda_stream))
+            a.top_n, a.out_top_ids = top_n, r.top_ids.data_ptr()
+            a.out_top_logprobs = r.top_logprobs.data_ptr()
+        if B == 0:
+            return r
+        rc = self._lib.llmk_logprobs(self._h, ctypes.byref(a), _raw_stream(self.device, stream))
         if rc != 0:
             raise SamplerError(rc, _lib.last_error())
-        self._keep(st, *[t for t in (r.logprobs, r.ranks, r.top_ids, r.top_logprobs) if t is not None])
+        if stream is not None:
+            for t in (r.logprobs, r.ranks, r.top_ids, r.top_logprobs):
+                if t is not None:
+                    t.record_stream(stream)
         return r
 
     def copy_pages(self, pools: "PagePools", src: torch.Tensor, dst: torch.Tensor,
                    stream: Optional[torch.cuda.Stream] = None) -> None:
         """llmk_pages_copy: page src[i] to page dst[i] in every pool.  The
         destinations must be distinct, and none of them a source."""
-        _on_device(pools.addresses.device, src=src, dst=dst)
+        self._same_device(pools.addresses)
+        if src.get_device() != self.device or dst.get_device() != self.device:
+            _on_device(pools.addresses.device, src=src, dst=dst)
         _flat("src", src, _U32)
         _flat("dst", dst, _U32)
-        self._same_device(pools.addresses.device)
         if src.numel() != dst.numel():
             raise SamplerError(_lib.LLMK_ERR_INVALID_ARGUMENT, "src and dst differ in length")
-        st = self._stream(src, stream)
-        rc = self._lib.llmk_pages_copy(self._h, pools.count, _ptr(pools.addresses),
+        rc = self._lib.llmk_pages_copy(self._h, pools.count, pools.addresses.data_ptr(),
                                        pools.page_bytes, pools.num_pages, src.numel(),
                                        src.data_ptr(), dst.data_ptr(),
-                                       ctypes.c_void_p(st.cuda_stream))
+                                       _raw_stream(self.device, stream))
         if rc != 0:
             raise SamplerError(rc, _lib.last_error())
 

@@ -4,7 +4,8 @@
 //! the `hip-sampler` feature.
 
 use std::ffi::c_void;
-use llm_kernel::hip_sampler::{HipSampler, LlmkSampleBatchArgs, LLMK_ERR_INVALID_ARGUMENT};
+use llm_kernel::hip_sampler::{HipSampler, LlmkLogprobsArgs, LlmkPageCache, LlmkProcessLogitsArgs,
+                               LlmkSampleBatchArgs, LLMK_ERR_INVALID_ARGUMENT};
 
 /// A sampler on `device` for batches up to `max_batch` rows of up to
 /// `max_vocab` logits; null on failure.
@@ -50,6 +51,53 @@ pub unsafe extern "C" fn llm_verify_batch(sampler: *mut c_void, batch: u32, voca
     let s = &*(sampler as *const HipSampler);
     match s.verify_batch(batch, vocab, ids, probs, list_cap, counts, draft_tokens, draft_probs,
                          draft_stride, u_accept, u_resample, out_tokens, out_accepted, stream) {
+        Ok(()) => 0,
+        Err(e) => e.code,
+    }
+}
+
+/// Processed logits (see `HipSampler::process_logits`): 0 on success, else the
+/// error code.
+/// # SAFETY: as llm_sample_batch.
+#[no_mangle]
+pub unsafe extern "C" fn llm_process_logits(sampler: *mut c_void, args: *const LlmkProcessLogitsArgs,
+                                            stream: *mut c_void) -> i32 {
+    if sampler.is_null() || args.is_null() {
+        return LLMK_ERR_INVALID_ARGUMENT;
+    }
+    match (*(sampler as *const HipSampler)).process_logits(&*args, stream) {
+        Ok(()) => 0,
+        Err(e) => e.code,
+    }
+}
+
+/// Log-probabilities (see `HipSampler::logprobs`): 0 on success, else the
+/// error code.
+/// # SAFETY: as llm_sample_batch.
+#[no_mangle]
+pub unsafe extern "C" fn llm_logprobs(sampler: *mut c_void, args: *const LlmkLogprobsArgs,
+                                      stream: *mut c_void) -> i32 {
+    if sampler.is_null() || args.is_null() {
+        return LLMK_ERR_INVALID_ARGUMENT;
+    }
+    match (*(sampler as *const HipSampler)).logprobs(&*args, stream) {
+        Ok(()) => 0,
+        Err(e) => e.code,
+    }
+}
+
+/// One step of a paged cache's rows (see `HipSampler::pages_update`): 0 on
+/// success, else the error code.
+/// # SAFETY: as llm_sample_batch; the cache's arrays are device memory.
+#[no_mangle]
+pub unsafe extern "C" fn llm_pages_update(sampler: *mut c_void, cache: *const LlmkPageCache,
+                                          parents: *const i32, new_lengths: *const i32,
+                                          out_granted: *mut u32, stream: *mut c_void) -> i32 {
+    if sampler.is_null() || cache.is_null() {
+        return LLMK_ERR_INVALID_ARGUMENT;
+    }
+    let s = &*(sampler as *const HipSampler);
+    match s.pages_update(&*cache, parents, new_lengths, out_granted, stream) {
         Ok(()) => 0,
         Err(e) => e.code,
     }

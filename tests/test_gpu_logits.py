@@ -204,8 +204,9 @@ def check_process(sampler, case, dtype, out="f32", pad=0, offset=0, inplace=Fals
     g = got.double().cpu().numpy()
     inf = np.isinf(want)
     assert np.array_equal(g[inf], want[inf])
-    bad = np.abs(g - want)[~inf] > tol[~inf]
-    assert not bad.any(), (np.abs(g - want)[~inf][bad][:5], tol[~inf][bad][:5])
+    off, tol = np.abs(g[~inf] - want[~inf]), tol[~inf]
+    bad = off > tol
+    assert not bad.any(), (off[bad][:5], tol[bad][:5])
     # nothing outside the rows is written
     mark = torch.ones(obuf.numel(), dtype=torch.bool, device="cuda:0")
     mark.as_strided((case.B, case.V), (case.V + pad, 1), offset).fill_(False)
@@ -594,3 +595,77 @@ def test_process_a_segment_with_thousands_of_history_tokens(sampler, inplace):
     check_process(sampler, case, "f32", inplace=inplace)
     case = Case(np.random.default_rng(32), 80, 9000, hist=30000, T=not inplace)
     check_process(sampler, case, "bf16", "same", inplace=inplace)
+
+
+def test_empty_lists_and_batches(sampler):
+    """Histories, extra tokens and biases that hold nothing at all; no rows."""
+    lg = torch.randn(3, 1000, device="cuda:0")
+    none = torch.empty(0, dtype=torch.int32, device="cuda:0")
+    zeros = torch.zeros(4, dtype=torch.int32, device="cuda:0")
+    lb = llmk.LogitsBatch(logits=lg, hist_offsets=zeros, hist_tokens=none, hist_counts=none,
+                          extra_begin=zeros, extra_count=zeros, extra_tokens=none, bias_offsets=zeros,
+                          bias_tokens=none, bias_values=none.float(),
+                          repetition_penalty=torch.full((3,), 1.5, device="cuda:0"))
+    assert torch.equal(sampler.process_logits(lb), lg)
+    assert sampler.process_logits(llmk.LogitsBatch(logits=lg[:0])).shape == (0, 1000)
+    r = sampler.logprobs(lg[:0], none, top_n=3)
+    assert r.logprobs.shape == (0,) and r.top_ids.shape == (0, 3)
+    with pytest.raises(llmk.SamplerError, match="Empty"):
+        sampler.process_logits(llmk.LogitsBatch(logits=lg[:, :0]))
+    with pytest.raises(llmk.SamplerError, match="Empty"):
+        sampler.logprobs(lg[:, :0], zeros[:3])
+
+
+def test_a_bias_of_minus_infinity_bans_a_token(sampler):
+    """-inf as a bias, on a token of the history and off it; +inf and -inf on one
+    token are NaN; a NaN bias."""
+    lg = torch.ones(1, 50, device="cuda:0")
+    inf = float("inf")
+    lb = llmk.LogitsBatch(logits=lg, hist_offsets=dev([0, 2]), hist_tokens=dev([4, 5]),
+                          presence_penalty=dev([0.5], torch.float32), bias_offsets=dev([0, 5]),
+                          bias_tokens=dev([4, 9, 11, 11, 12]),
+                          bias_values=dev([-inf, -inf, inf, -inf, float("nan")], torch.float32))
+    g = sampler.process_logits(lb)[0].cpu()
+    assert g[4] == -inf and g[9] == -inf and g[5] == 0.5 and g[0] == 1
+    assert torch.isnan(g[[11, 12]]).all() and int(torch.isnan(g).sum()) == 2
+
+
+def test_two_calls_at_once(sampler):
+    """process_logits keeps nothing between the workgroups of a call: calls that
+    overlap on two streams do not disturb each other."""
+    cases = [Case(np.random.default_rng(40 + i), 64, 50000, hist=800, bias=30) for i in range(2)]
+    lbs = [c.batch(rows_on_device(c.lg, "f32")[1]) for c in cases]
+    alone = [sampler.process_logits(lb) for lb in lbs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [torch.empty_like(a) for a in alone]
+    for _ in range(5):
+        for lb, o, s in zip(lbs, outs, streams):
+            sampler.process_logits(lb, out=o, stream=s)
+    torch.cuda.synchronize()
+    for a, o in zip(alone, outs):
+        assert torch.equal(a, o)
+
+
+def test_two_graphs_of_one_handle(sampler):
+    """Two captured calls that share the handle's workspace, replayed in turn."""
+    lg = [torch.randn(5, 30000, device="cuda:0"), torch.randn(7, 50000, device="cuda:0").bfloat16()]
+    tok = [dev(np.arange(5)), dev(np.arange(7))]
+    graphs, outs = [], []
+    for x, t in zip(lg, tok):
+        sampler.logprobs(x, t, top_n=6)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(sampler.logprobs(x, t, top_n=6))
+        graphs.append(g)
+    for i in range(4):
+        for x in lg:
+            x.copy_(torch.randn(x.shape, device="cuda:0") * (i + 1))
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for x, t, r in zip(lg, tok, outs):
+            e = sampler.logprobs(x, t, top_n=6)
+            assert torch.equal(r.logprobs, e.logprobs) and torch.equal(r.ranks, e.ranks)
+            assert torch.equal(r.top_ids, e.top_ids) and torch.equal(r.top_logprobs, e.top_logprobs)

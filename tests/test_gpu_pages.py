@@ -361,3 +361,29 @@ def test_a_serving_step(sampler):
             seen[b].append(int(d.tokens[b]))
         assert np.array_equal(host(hist)[1, :host(lens)[1]], seen[1])
     s.close()
+
+
+def test_more_pages_than_the_words_kept_in_shared_memory(sampler):
+    """200000 pages (past 131072 their words stay in memory), rows of tens of
+    thousands of them (more than the list of free pages kept there), given up,
+    grown, moved."""
+    c = Pair(sampler, 6, 60000, 4, 200000, page_words=(8,))
+    c.update([4 * 40000, 4 * 30000 + 1, 17, 4 * 20000, -1, -1])
+    c.update([0, -1, 4 * 5000, -1, -1, -1])
+    c.update([-1, 4 * 30000 + 2, -1, 4 * 100, 4 * 30000 + 3, 4 * 50000], [-1, -1, -1, -1, 1, -1])
+    c.update([4 * 60000] * 6)
+    c.compact()
+    c.update([1, 2, 3, 4, 5, 6])
+    c.compact()
+
+
+@pytest.mark.parametrize("rows", [511, 512, 513])
+def test_rows_about_the_threads_of_a_workgroup(sampler, rows):
+    c = Pair(sampler, rows, 3, 4, 2 * rows, page_words=(8,))
+    c.update([(r * 7) % 13 for r in range(rows)])
+    new = c.plain.lengths + 1
+    new[::5] = 0
+    c.update(new)
+    par = np.where(c.plain.lengths == 0, 1, -1)
+    c.update(np.where(par >= 0, c.plain.lengths[1] + 1, -1), par)
+    c.compact()
