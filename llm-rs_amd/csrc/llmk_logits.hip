@@ -161,6 +161,7 @@ __device__ __forceinline__ void divide4(float* x, const Divisor& d) {
   }
 }
 
+constexpr uint32_t PT = 256;        // threads of process_kernel
 constexpr uint32_t TOUCHED = 2048;  // tokens listed per segment (below)
 
 // One workgroup per (row, segment of PT * N logits).  LDS holds a word per
@@ -173,24 +174,26 @@ constexpr uint32_t TOUCHED = 2048;  // tokens listed per segment (below)
 //
 // Bound by HBM without lists (512 x 128256 bf16 to bf16 47 us, 5.5 TB/s).  With
 // them by the steps before the last logit can be written: extents, tokens,
-// words, each a wait that only the CU's other three workgroups fill (with
-// histories of 1000 tokens 74 us; 256 x 151936 f32 with 2048 tokens 65 us,
-// 4.8 TB/s).  So the tokens are requested before the logits (loads come back
-// in order), barriers wait for LDS alone, and the penalties are computed where
-// the logits are, though that costs a wave an operation for each of its
-// logits as soon as one of the 64 neighbours has a count: a list of the touched
-// tokens, penalised by a thread each from memory, took 71 us instead of 65.
+// words, each a wait that only the CU's other seven workgroups fill (with
+// histories of 1000 tokens 66 us; 256 x 151936 f32 with 2048 tokens 60 us,
+// 5.2 TB/s).  So workgroups are small (512 threads for segments twice as long
+// took up to 8 % longer, 1024 threads 5 to 29 %, 128 threads up to 7 %), the
+// tokens are requested before the logits (loads come back in order), barriers
+// wait for LDS alone, and the penalties are computed where the logits are,
+// though that costs a wave an operation for each of its logits as soon as one
+// of the 64 neighbours has a count: a list of the touched tokens, penalised by
+// a thread each from memory, took 9 % longer.
 // TOUCHED_ONLY, for calls in place that change no other logit (no softcap, bias,
 // mask or temperature), has such a list, and reads and writes nothing else.
 // Fewer, longer workgroups that run over several segments with the next one's
 // logits on their way took 90 us: fewer of them fit a CU.  The segments of a
 // row re-read its lists from L2, so they share an XCD.
-template <int DT, int OT, uint32_t PT, bool TOUCHED_ONLY>
+template <int DT, int OT, uint32_t N, bool TOUCHED_ONLY>
 __global__ __launch_bounds__(PT, 8) void process_kernel(PArgs a) {
   extern __shared__ uint32_t psm[];
   __shared__ uint16_t s_list[TOUCHED_ONLY ? TOUCHED : 1];
   __shared__ uint32_t s_listed, s_twice;
-  constexpr uint32_t W = Elem<DT>::W, N = PT == 512 ? 16 : 8, CH = N / W, SEG = PT * N;
+  constexpr uint32_t W = Elem<DT>::W, CH = N / W, SEG = PT * N;
   const uint32_t tid = threadIdx.x;
   uint32_t b, g;
   if ((a.B & 7u) == 0) {  // blocks go round the 8 XCDs: a row's segments on one
@@ -909,11 +912,11 @@ extern "C" int llmk_process_logits(llmk_sampler* s, const llmk_process_logits_ar
   if (!rows_apart(in))
     return fail(LLMK_ERR_INVALID_ARGUMENT,
                 "out overlaps logits: in place needs the same address, dtype and stride");
-  // Segments of 8192 logits where that makes two workgroups per CU or more,
+  // Segments of 4096 logits where that makes four workgroups per CU or more,
   // of 2048 where it does not.
-  const uint32_t big = 8192, small = 2048;
-  const bool large = (uint64_t)in->batch * ((in->vocab + big - 1) / big) >= 512;
-  const uint32_t seg = large ? big : small;
+  constexpr uint32_t big = 16, small = 8;  // logits per thread
+  const bool large = (uint64_t)in->batch * ((in->vocab + big * PT - 1) / (big * PT)) >= 1024;
+  const uint32_t seg = (large ? big : small) * PT;
   const uint32_t nseg = (in->vocab + seg - 1) / seg;
   const uint64_t blocks = (uint64_t)in->batch * nseg;
   if (blocks > 0x7fffffffu) return fail(LLMK_ERR_CAPACITY, "batch * vocab too large for one call");
@@ -955,17 +958,17 @@ extern "C" int llmk_process_logits(llmk_sampler* s, const llmk_process_logits_ar
   const bool touched_only = in->out == in->logits && !sc && !in->temperature && !in->allow_mask &&
                             !in->bias_offsets;
   auto launch = [&](auto kern) {
-    hipLaunchKernelGGL(kern, dim3((uint32_t)blocks), dim3(large ? 512 : 256), lds,
+    hipLaunchKernelGGL(kern, dim3((uint32_t)blocks), dim3(PT), lds,
                        (hipStream_t)stream, a);
   };
-#define LLMK_PROCESS(DT, OT)                                                   \
-  do {                                                                         \
-    if (touched_only && large) launch(process_kernel<DT, DT, 512, true>);      \
-    else if (touched_only) launch(process_kernel<DT, DT, 256, true>);          \
-    else if (sc && large) launch(process_kernel<(DT) | SOFTCAP, OT, 512, false>); \
-    else if (sc) launch(process_kernel<(DT) | SOFTCAP, OT, 256, false>);       \
-    else if (large) launch(process_kernel<DT, OT, 512, false>);                \
-    else launch(process_kernel<DT, OT, 256, false>);                           \
+#define LLMK_PROCESS(DT, OT)                                                      \
+  do {                                                                            \
+    if (touched_only && large) launch(process_kernel<DT, DT, big, true>);         \
+    else if (touched_only) launch(process_kernel<DT, DT, small, true>);           \
+    else if (sc && large) launch(process_kernel<(DT) | SOFTCAP, OT, big, false>); \
+    else if (sc) launch(process_kernel<(DT) | SOFTCAP, OT, small, false>);        \
+    else if (large) launch(process_kernel<DT, OT, big, false>);                   \
+    else launch(process_kernel<DT, OT, small, false>);                            \
   } while (0)
   if (in->dtype == LLMK_F32) LLMK_PROCESS(LLMK_F32, LLMK_F32);
   else if (in->dtype == LLMK_BF16 && in->out_dtype == LLMK_F32) LLMK_PROCESS(LLMK_BF16, LLMK_F32);

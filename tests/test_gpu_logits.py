@@ -597,6 +597,22 @@ def test_process_a_segment_with_thousands_of_history_tokens(sampler, inplace):
     check_process(sampler, case, "bf16", "same", inplace=inplace)
 
 
+@pytest.mark.parametrize("dtype,out", [("f32", "f32"), ("bf16", "f32"), ("bf16", "same"),
+                                       ("f16", "f32"), ("f16", "same")])
+@pytest.mark.parametrize("B,softcap", [(1041, 0.0), (528, 25.0)])
+def test_process_many_rows(sampler, dtype, out, B, softcap):
+    """Enough rows for long segments, with rows in eights and not."""
+    case = Case(np.random.default_rng(B), B, 5003, chain=1 if softcap else 3, hist=600, bias=40, mask=True,
+                softcap=softcap)
+    check_process(sampler, case, dtype, out, 1, 1)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_process_many_rows_in_place_with_full_lists(sampler, dtype):
+    case = Case(np.random.default_rng(33), 520, 4500, hist=12000, T=False)
+    check_process(sampler, case, dtype, "same", inplace=True)
+
+
 def test_empty_lists_and_batches(sampler):
     """Histories, extra tokens and biases that hold nothing at all; no rows."""
     lg = torch.randn(3, 1000, device="cuda:0")
