@@ -29,13 +29,11 @@ MALL_BYTES = 256 << 20
 def kernel_source_digest():
     """sha256 of the sampling kernels' sources: a traffic summary applies to
     the kernels it was measured on and to no later edit."""
-    import glob
     import hashlib
     h = hashlib.sha256()
-    for path in sorted(glob.glob(os.path.join(ROOT, "llm-rs_amd", "csrc", "llmk_*"))):
-        if "read_probe" not in path:
-            with open(path, "rb") as f:
-                h.update(f.read())
+    for name in ("llmk_device.h", "llmk_numerics.h", "llmk_sampler.hip"):
+        with open(os.path.join(ROOT, "llm-rs_amd", "csrc", name), "rb") as f:
+            h.update(f.read())
     return h.hexdigest()
 
 
