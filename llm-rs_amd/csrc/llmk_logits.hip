@@ -24,6 +24,7 @@ namespace llmk {
 // gfx950's global memory instructions take unaligned addresses.
 typedef uint32_t u4v_a4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u4v_a2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u2v_a2 __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint32_t u4v_list __attribute__((ext_vector_type(4), aligned(4)));
 
 template <int DT>
@@ -32,14 +33,17 @@ struct Elem {
   static constexpr uint32_t W = 16 / SZ;  // logits per 16 bytes
 };
 
-// The W logits from element e of a row of V, packed; elements past V read as
-// zero bits.  e < V.
-template <int DT>
+// The W logits from element e of a row of V, packed (W = 4 of 16 bits: the
+// first two words); elements past V read as zero bits.  e < V.
+template <int DT, uint32_t W = Elem<DT>::W>
 __device__ __forceinline__ u4v load_pack(const void* row, uint32_t e, uint32_t V) {
-  constexpr uint32_t W = Elem<DT>::W;
   if (e + W <= V) {
     if (Elem<DT>::SZ == 4)
       return (u4v)__builtin_nontemporal_load((const GLB u4v_a4*)G((const uint32_t*)row + e));
+    if (W == 4) {
+      const u2v p = (u2v)__builtin_nontemporal_load((const GLB u2v_a2*)G((const uint16_t*)row + e));
+      return u4v{p[0], p[1], 0, 0};
+    }
     return (u4v)__builtin_nontemporal_load((const GLB u4v_a2*)G((const uint16_t*)row + e));
   }
   u4v r = {0, 0, 0, 0};
@@ -99,8 +103,8 @@ struct PArgs {
 // [0, 1] (off by 1.4 units with the rounding of its steps).  From 1 on:
 // 1 - 2 / (1 + e^2z), whose error of 6.5 units falls on a difference from 1 of
 // at most 0.24.  (glibc's steps, which llmk_sample_batch repeats bit for bit,
-// take about four times the operations: 256 x 128256 bf16 with a softcap 95 us
-// with those instead of 44.)
+// take about four times the operations: 256 x 128256 bf16 to f32 with a softcap
+// takes 40 us with these, and took 51 longer with those.)
 __device__ __forceinline__ float tanh_f32(float z) {
   const float a = __builtin_fabsf(z), s = z * z;
   float q = -0x1.bc54ap-12f;
@@ -193,7 +197,10 @@ __global__ __launch_bounds__(PT, 8) void process_kernel(PArgs a) {
   extern __shared__ uint32_t psm[];
   __shared__ uint16_t s_list[TOUCHED_ONLY ? TOUCHED : 1];
   __shared__ uint32_t s_listed, s_twice;
-  constexpr uint32_t W = Elem<DT>::W, CH = N / W, SEG = PT * N;
+  // 16 bytes a lane from memory or, where the results are wider, to it: then a
+  // wave's stores fill lines (512 x 128257 bf16 to f32 75 us; 83 with 16 bytes
+  // read a lane, whose 32 bytes go out in two halves).
+  constexpr uint32_t W = OT == LLMK_F32 ? 4 : Elem<DT>::W, CH = N / W, SEG = PT * N;
   const uint32_t tid = threadIdx.x;
   uint32_t b, g;
   if ((a.B & 7u) == 0) {  // blocks go round the 8 XCDs: a row's segments on one
@@ -259,10 +266,8 @@ __global__ __launch_bounds__(PT, 8) void process_kernel(PArgs a) {
   uint32_t mw[CH];
   if (mrow) {
 #pragma unroll
-    for (uint32_t c = 0; c < CH; ++c) {
-      const uint32_t e = lo + (c * PT + tid) * W;
-      mw[c] = e < a.V ? G(mrow)[e >> 5] >> (e & 31u) : 0u;  // W divides 32
-    }
+    for (uint32_t c = 0; c < CH; ++c)  // (no lane skips a load: it would be waited for here)
+      mw[c] = G(mrow)[umin(lo + (c * PT + tid) * W, a.V - 1) >> 5];
   }
   u4v r[CH];
   auto request = [&]() {
@@ -270,7 +275,7 @@ __global__ __launch_bounds__(PT, 8) void process_kernel(PArgs a) {
     for (uint32_t c = 0; c < CH; ++c) {
       const uint32_t e = lo + (c * PT + tid) * W;
       r[c] = u4v{0, 0, 0, 0};
-      if (e < a.V) r[c] = load_pack<DT>(row, e, a.V);
+      if (e < a.V) r[c] = load_pack<DT, W>(row, e, a.V);
     }
   };
   if (!TOUCHED_ONLY) request();
@@ -308,15 +313,19 @@ __global__ __launch_bounds__(PT, 8) void process_kernel(PArgs a) {
       lds_barrier();
     }
 #pragma unroll
-    for (uint32_t i = 0; i < N; ++i) {
-      const uint32_t t = ((i / W) * PT + tid) * W + i % W, w = cnt[t];
-      add[i] = w == EMPTY ? 0.0f : __uint_as_float(w);
-      if (w == EMPTY) continue;
-      cnt[t] = EMPTY;  // for the counts
-      if (twice) {
-        add[i] = G(bv)[w];
-        for (uint32_t k = w + 1; k < nb; ++k)
-          if (G(bt)[k] == lo + t) add[i] += G(bv)[k];
+    for (uint32_t h = 0; h < N; h += 4) {
+      const uint32_t at = ((h / W) * PT + tid) * W + h % W;
+      const u4v m = *(LDS u4v*)(cnt + at);
+#pragma unroll
+      for (uint32_t k = 0; k < 4; ++k) {
+        add[h + k] = m[k] == EMPTY ? 0.0f : __uint_as_float(m[k]);
+        if (m[k] == EMPTY) continue;
+        cnt[at + k] = EMPTY;  // for the counts
+        if (twice) {
+          add[h + k] = G(bv)[m[k]];
+          for (uint32_t j = m[k] + 1; j < nb; ++j)
+            if (G(bt)[j] == lo + at + k) add[h + k] += G(bv)[j];
+        }
       }
     }
     lds_barrier();
@@ -399,7 +408,7 @@ __global__ __launch_bounds__(PT, 8) void process_kernel(PArgs a) {
     if (mrow) {
 #pragma unroll
       for (uint32_t k = 0; k < W; ++k)
-        if (!((mw[c] >> k) & 1u)) x[k] = NEG_INF;
+        if (!((mw[c] >> ((e & 31u) + k)) & 1u)) x[k] = NEG_INF;  // W divides 32
     }
     if (e + W <= a.V) {
       if (OT == LLMK_F32) {
