@@ -66,6 +66,29 @@ __device__ __forceinline__ uint64_t update_scan(uint32_t x, LDS uint32_t* red, u
   return off + incl - x;
 }
 
+// The same of y, with the sum of x beside it.
+__device__ __forceinline__ uint64_t update_scan_and_sum(uint32_t y, uint32_t x, LDS uint32_t* red,
+                                                        uint64_t& total, uint64_t& sum_x) {
+  const uint32_t lane = threadIdx.x & 63u, wv = threadIdx.x >> 6;
+  const uint32_t incl = wave_incl_scan(y), all = wave_incl_scan(x);
+  if (lane == 63) {
+    red[wv] = incl;
+    red[UW + wv] = all;
+  }
+  lds_barrier();
+  uint64_t off = 0, sum = 0, xs = 0;
+#pragma unroll
+  for (uint32_t i = 0; i < UW; ++i) {
+    off += i < wv ? red[i] : 0u;
+    sum += red[i];
+    xs += red[UW + i];
+  }
+  lds_barrier();
+  total = sum;
+  sum_x = xs;
+  return off + incl - y;
+}
+
 // What a row asks for, as its workgroup leaves it for the last one, and the
 // counts at the page it marked.
 struct Request {
@@ -120,12 +143,16 @@ __device__ __forceinline__ Request request_of(const Cache& c, uint32_t r) {
 // counts of shared pages change only when every row has read them; of the rows
 // that share a page and all grow, the last keeps it.
 //
-// Bound by latency: a few dependent rounds of loads and one arrival (256 rows,
-// 64 K pages: 10 us; as four launches with whole-device fences between them 29).
+// Bound by latency, 256 rows of 80 K pages 18 us: 5 until every row has arrived,
+// 5 for what the last workgroup reads and for the pages given up, 3 for sums and
+// the list of free pages, 5 for the rows' shares.  (As four launches 33 us; the
+// sums of pages and rows apart, and the words without the taken pages in a pass
+// of their own, 20.)  Reading more freed pages at once, spreading them over the
+// lanes and smaller code changed nothing.
 __global__ __launch_bounds__(UT) void pages_update_kernel(Cache c, const int32_t* parents,
                                                           const int32_t* new_lengths,
                                                           uint32_t* granted, uint32_t* status) {
-  __shared__ uint32_t s_red[UW], s_job[UT][4], s_free[FREE_LDS], s_word[FREE_LDS];
+  __shared__ uint32_t s_red[2 * UW], s_job[UT][4], s_free[FREE_LDS], s_word[FREE_LDS];
   __shared__ uint32_t s_jobs, s_moves, s_taken, s_last;
   LDS uint32_t* red = (LDS uint32_t*)s_red;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wv = tid >> 6;
@@ -237,7 +264,7 @@ __global__ __launch_bounds__(UT) void pages_update_kernel(Cache c, const int32_t
 #pragma unroll
     for (uint32_t k = 0; k < WB; ++k)
       if (k * UT + tid < c.words) s_word[k * UT + tid] = page_bits(c, k * UT + tid) & ~word[k];
-  if (tid == 0) s_moves = s_taken = 0;
+  if (tid == 0) s_moves = s_taken = s_jobs = 0;
   lds_barrier();
   auto give_up = [&](uint32_t page) {
     const uint32_t w = page >> 5, bit = 1u << (page & 31u);
@@ -262,30 +289,32 @@ __global__ __launch_bounds__(UT) void pages_update_kernel(Cache c, const int32_t
   };
   uint32_t here = 0;
   for (uint32_t w = tid; w < c.words; w += UT) here += __popc(free_word(w));
-  uint64_t nfree = 0, asked = 0;
-  (void)update_scan(here, red, nfree);
-  // how many pages all the rows ask for: no more free ones than that are listed
-  const uint32_t cap = (uint32_t)nfree + 1;
-  for (uint32_t r0 = 0; r0 < c.rows; r0 += UT) {
-    uint64_t sum = 0;
-    const uint32_t need = one ? mine.need : (r0 + tid < c.rows ? request_of(c, r0 + tid).need : 0u);
-    (void)update_scan(umin(need, cap), red, sum);
-    asked += sum;
+  // How many pages all the rows ask for: no more free ones than that are listed.
+  // (A row that asks for more than there are gets none, nor does one after it.)
+  const uint32_t cap = c.num_pages + 1;
+  uint64_t nfree = 0, asked = 0, mine_first = 0;
+  if (one) {
+    mine_first = update_scan_and_sum(umin(mine.need, cap), here, red, asked, nfree);
+  } else {
+    (void)update_scan(here, red, nfree);
+    for (uint32_t r0 = 0; r0 < c.rows; r0 += UT) {
+      uint64_t sum = 0;
+      const uint32_t need = r0 + tid < c.rows ? request_of(c, r0 + tid).need : 0u;
+      (void)update_scan(umin(need, cap), red, sum);
+      asked += sum;
+    }
   }
   const uint32_t listed = (uint32_t)(asked < nfree ? asked : nfree);
   const bool in_lds = listed <= FREE_LDS;
-  // the words of a round, a thread each: f(word, its free pages, how many lie before)
-  auto words_below = [&](uint32_t many, auto f) {
-    uint32_t base = 0;
-    for (uint32_t w0 = 0; w0 < c.words && base < many; w0 += UT) {
-      const uint32_t m = free_word(w0 + tid);
-      uint64_t sum = 0;
-      const uint32_t from = base + (uint32_t)update_scan(__popc(m), red, sum);
-      base += (uint32_t)sum;
-      f(w0 + tid, m, from);
-    }
-  };
-  words_below(listed, [&](uint32_t w, uint32_t m, uint32_t at) {
+  // the listed pages, and the words without them, a round of words at a time
+  uint32_t base = 0;
+  for (uint32_t w0 = 0; w0 < c.words && base < listed; w0 += UT) {
+    const uint32_t w = w0 + tid;
+    uint32_t m = free_word(w);
+    uint64_t sum = 0;
+    uint32_t at = base + (uint32_t)update_scan(__popc(m), red, sum);
+    base += (uint32_t)sum;
+    if (m == 0 || at >= listed) continue;
     for (; m && at < listed; m &= m - 1, ++at) {
       const uint32_t page = 32 * w + (uint32_t)__builtin_ctz(m);
       if (in_lds)
@@ -293,7 +322,13 @@ __global__ __launch_bounds__(UT) void pages_update_kernel(Cache c, const int32_t
       else
         put_agent(c.list + at, page);
     }
-  });
+    if (few)
+      s_word[w] = m;
+    else
+      put_agent(c.used + w, page_bits(c, w) & ~m);
+  }
+  if (!in_lds || !few) wait_stores();
+  lds_barrier();
   auto free_page = [&](uint32_t k) { return in_lds ? s_free[k] : get_agent(c.list + k); };
 
   uint64_t total = 0;  // pages asked for by the rows so far
@@ -301,10 +336,11 @@ __global__ __launch_bounds__(UT) void pages_update_kernel(Cache c, const int32_t
     const uint32_t r = r0 + tid;
     Request q = mine;
     if (!one) q = r < c.rows ? request_of(c, r) : no_request();
-    if (tid == 0) s_jobs = 0;
-    uint64_t sum = 0;
-    if (!in_lds) wait_stores();  // the list
-    const uint64_t first = total + update_scan(umin(q.need, cap), red, sum);
+    uint64_t sum = 0, first = mine_first;
+    if (!one) {
+      if (tid == 0) s_jobs = 0;
+      first = total + update_scan(umin(q.need, cap), red, sum);
+    }
     bool grow = q.want != EMPTY;
     if (grow && first + q.need > nfree && (q.need || q.tied)) {
       put_agent(granted + r, 0u);
@@ -345,17 +381,13 @@ __global__ __launch_bounds__(UT) void pages_update_kernel(Cache c, const int32_t
     total += sum;
     lds_barrier();  // the jobs are read
   }
-  // the words of `used`: the first s_taken free pages are in use now
+  // listed pages that no row got are free again
   const uint32_t taken = s_taken;
-  words_below(taken, [&](uint32_t w, uint32_t m, uint32_t at) {
-    if (m == 0) return;
-    for (; m && at < taken; ++at) m &= m - 1;
-    if (few)
-      s_word[w] = m;
-    else
-      put_agent(c.used + w, page_bits(c, w) & ~m);
-  });
-  if (few && (taken || nfreed))  // (each thread the words it wrote)
+  if (taken < listed) {
+    for (uint32_t i = taken + tid; i < listed; i += UT) give_up(free_page(i));
+    lds_barrier();
+  }
+  if (few && (taken || nfreed))
     for (uint32_t w = tid; w < c.words; w += UT) put_agent(c.used + w, page_bits(c, w) & ~s_word[w]);
   // the copied pages lose the rows that left them; what calls begin with
   __syncthreads();  // (the moves are written)
@@ -448,7 +480,7 @@ struct Copies {
 
 // Work items are (pair, pool, piece of CPIECE bytes), taken in turn by the
 // workgroups `first` on: the number of pairs may be known on the device alone.
-// Bound by HBM, read and written: 4000 pages of 32 KiB in 4 pools 216 us, 4.9
+// Bound by HBM, read and written: 4000 pages of 32 KiB in 4 pools 215 us, 4.9
 // TB/s, as a copy of as many bytes in one piece.
 constexpr uint32_t CT = 256, CPIECE = CT * 16 * 4;
 __device__ __forceinline__ void copy_items(const Copies& a, uint32_t first) {
