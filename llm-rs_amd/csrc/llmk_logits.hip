@@ -546,10 +546,10 @@ struct Tile16 {
 // descending, index ascending): a token of any other tile has the top_n
 // maxima of those before it.  So the stream carries no list; the last
 // workgroup reads top_n tiles again and picks from them.  (A list of
-// candidates kept by every wave took 90 us instead of 31 for 256 x 151936 f32
+// candidates kept by every wave took 90 us instead of 30 for 256 x 151936 f32
 // with a list of 8.)
 //
-// Bound by HBM: that call reads its 156 MB at 5.0 TB/s, without a list at 5.5
+// Bound by HBM: that call reads its 156 MB at 5.2 TB/s, without a list at 5.7
 // TB/s.  64 registers, so that 8 waves fit a SIMD (2047 x 32000 f16 with a
 // list of 1: 35 us with 80 registers, 31.6 with 64); the last steps are kept in
 // short loops, since their code comes from L2 when a workgroup first gets there.

@@ -145,7 +145,7 @@ __device__ __forceinline__ Request request_of(const Cache& c, uint32_t r) {
 //
 // Bound by latency, 256 rows of 80 K pages 18 us: 5 until every row has arrived,
 // 5 for what the last workgroup reads and for the pages given up, 3 for sums and
-// the list of free pages, 5 for the rows' shares.  (As four launches 33 us; the
+// the list of free pages, 5 for the rows' shares.  (As four launches 29 us; the
 // sums of pages and rows apart, and the words without the taken pages in a pass
 // of their own, 20.)  Reading more freed pages at once, spreading them over the
 // lanes and smaller code changed nothing.
