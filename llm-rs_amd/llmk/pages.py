@@ -16,7 +16,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from .sampler import _I32, HipSampler, SamplerError, _flat, _on_device, _ptr, _raw_stream
+from .sampler import _I32, HipSampler, SamplerError, _flat, _on_device, _output, _ptr, _raw_stream
 
 
 class PagePools:
@@ -127,22 +127,18 @@ class PageCache:
             _flat(name, t, _I32)
             if t.numel() != self.rows:
                 raise SamplerError(_lib.LLMK_ERR_INVALID_ARGUMENT, f"{name} needs an entry per row")
-        granted = torch.empty(self.rows, dtype=torch.int32, device=self.state.device)
+        granted = _output(stream, self.rows, dtype=torch.int32, device=self.state.device)
         self._check(self._lib.llmk_pages_update(
             self.sampler._h, ctypes.byref(self._args), _ptr(parents), _ptr(new_lengths),
             granted.data_ptr(), self._stream(stream)))
-        if stream is not None:
-            granted.record_stream(stream)
         return granted
 
     def compact(self, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
         """llmk_pages_compact: the pages in use move to the front.  Returns
         int32 [num_pages]: where each page's contents are now."""
-        out = torch.empty(self.num_pages, dtype=torch.int32, device=self.state.device)
+        out = _output(stream, self.num_pages, dtype=torch.int32, device=self.state.device)
         self._check(self._lib.llmk_pages_compact(self.sampler._h, ctypes.byref(self._args),
                                                  out.data_ptr(), self._stream(stream)))
-        if stream is not None:
-            out.record_stream(stream)
         return out
 
     def copy(self, src: torch.Tensor, dst: torch.Tensor,

@@ -254,6 +254,20 @@ def _raw_stream(device: int, stream: Optional[torch.cuda.Stream]) -> int:
     return _current_raw(device) if _current_raw else torch.cuda.current_stream(device).cuda_stream
 
 
+def _output(stream: Optional[torch.cuda.Stream], *shape: int, dtype: torch.dtype,
+            device: torch.device) -> torch.Tensor:
+    """A new output of a call on `stream` (None: the current one).  It is of that
+    stream's memory: a block that was freed on the current one may still be in
+    use there.  The current one, where it is read as a rule, keeps it as well."""
+    if stream is None:
+        return torch.empty(*shape, dtype=dtype, device=device)
+    current = torch.cuda.current_stream(device)
+    with torch.cuda.stream(stream):
+        t = torch.empty(*shape, dtype=dtype, device=device)
+    t.record_stream(current)
+    return t
+
+
 def _batch_args(db: DeviceBatch, out_tokens: torch.Tensor,
                 out_ids: Optional[torch.Tensor], out_probs: Optional[torch.Tensor],
                 out_count: Optional[torch.Tensor]) -> "_lib.SampleBatchArgs":
@@ -583,11 +597,10 @@ class HipSampler:
         """llmk_process_logits: softcap, logit bias, penalties, allow-mask and
         temperature of every row, into `out` ([B, >= V], float32 or the logits'
         dtype; lb.logits itself: in place), by default a new float32 tensor."""
-        new = out is None
-        if new:
+        if out is None:
             _logits_rows("logits", lb.logits)
-            out = torch.empty(lb.logits.shape[0], _vocab(lb.logits, lb.vocab), dtype=torch.float32,
-                              device=lb.logits.device)
+            out = _output(stream, lb.logits.shape[0], _vocab(lb.logits, lb.vocab),
+                          dtype=torch.float32, device=lb.logits.device)
         a = _process_args(lb, out)
         self._same_device(lb.logits)
         if a.batch == 0:
@@ -595,8 +608,6 @@ class HipSampler:
         rc = self._lib.llmk_process_logits(self._h, ctypes.byref(a), _raw_stream(self.device, stream))
         if rc != 0:
             raise SamplerError(rc, _lib.last_error())
-        if new and stream is not None:
-            out.record_stream(stream)
         return out
 
     def logprobs(self, logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
@@ -618,13 +629,13 @@ class HipSampler:
                 _on_device(dev, tokens=tokens)
             _flat("tokens", tokens, _U32)
             _entries("tokens", tokens, B)
-            r.logprobs = torch.empty(B, dtype=torch.float32, device=dev)
-            r.ranks = torch.empty(B, dtype=torch.int32, device=dev)
+            r.logprobs = _output(stream, B, dtype=torch.float32, device=dev)
+            r.ranks = _output(stream, B, dtype=torch.int32, device=dev)
             a.tokens, a.out_logprobs = tokens.data_ptr(), r.logprobs.data_ptr()
             a.out_ranks = r.ranks.data_ptr()
         if top_n:
-            r.top_ids = torch.empty(B, top_n, dtype=torch.int32, device=dev)
-            r.top_logprobs = torch.empty(B, top_n, dtype=torch.float32, device=dev)
+            r.top_ids = _output(stream, B, top_n, dtype=torch.int32, device=dev)
+            r.top_logprobs = _output(stream, B, top_n, dtype=torch.float32, device=dev)
             a.top_n, a.out_top_ids = top_n, r.top_ids.data_ptr()
             a.out_top_logprobs = r.top_logprobs.data_ptr()
         if B == 0:
@@ -632,10 +643,6 @@ class HipSampler:
         rc = self._lib.llmk_logprobs(self._h, ctypes.byref(a), _raw_stream(self.device, stream))
         if rc != 0:
             raise SamplerError(rc, _lib.last_error())
-        if stream is not None:
-            for t in (r.logprobs, r.ranks, r.top_ids, r.top_logprobs):
-                if t is not None:
-                    t.record_stream(stream)
         return r
 
     def copy_pages(self, pools: "PagePools", src: torch.Tensor, dst: torch.Tensor,

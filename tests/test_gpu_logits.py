@@ -535,6 +535,30 @@ def test_another_stream(sampler):
     assert torch.equal(a, out) and torch.equal(ra.logprobs, rb.logprobs) and torch.equal(ra.top_ids, rb.top_ids)
 
 
+def test_outputs_of_another_stream_take_no_block_in_use(sampler):
+    """A block freed on the current stream while work that reads it waits there
+    is not what a call on another stream writes its results to."""
+    B, V = 64, 50001
+    lg, tok = torch.randn(B, V, device="cuda:0"), torch.zeros(B, dtype=torch.int32, device="cuda:0")
+    cache = llmk.PageCache(sampler, B, 4, 16, 50001)
+    grown = torch.ones(B, dtype=torch.int32, device="cuda:0")
+    s = torch.cuda.Stream()
+    calls = ((B * V, lambda: sampler.process_logits(llmk.LogitsBatch(logits=lg), stream=s)),
+             (B * 20, lambda: sampler.logprobs(lg, tok, top_n=20, stream=s)),
+             (B, lambda: cache.update(new_lengths=grown, stream=s)),
+             (50001, lambda: cache.compact(stream=s)))
+    for n, call in calls:
+        x = torch.full((n,), 5.0, device="cuda:0")
+        torch.cuda.synchronize()
+        torch.cuda._sleep(20_000_000)
+        y = x.clone()
+        del x
+        r = call()
+        torch.cuda.synchronize()
+        assert bool((y == 5.0).all())
+        del r
+
+
 def test_rows_past_32_bit_offsets(sampler):
     """A row stride of more than 2^31 elements (bf16: 4 GiB from row to row)."""
     V, stride = 3001, 2**31 + 8
