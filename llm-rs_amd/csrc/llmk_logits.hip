@@ -522,13 +522,10 @@ struct Tile16 {
   static __device__ __forceinline__ uint32_t index(uint32_t t, uint32_t i) {
     return t * TILE + ((i / W) * 64 + (threadIdx.x & 63u)) * W + i % W;
   }
-  // as floats, NaN and what lies past V as -inf
+  // as floats, what lies past V as -inf
   __device__ __forceinline__ void values(uint32_t t, uint32_t V, float (&x)[16]) const {
 #pragma unroll
-    for (uint32_t i = 0; i < 16; ++i) {
-      x[i] = unpack<DT>(raw[i / W], i % W);
-      if (!(x[i] == x[i])) x[i] = NEG_INF;
-    }
+    for (uint32_t i = 0; i < 16; ++i) x[i] = unpack<DT>(raw[i / W], i % W);
     if (t * TILE + TILE > V) {
 #pragma unroll
       for (uint32_t i = 0; i < 16; ++i)
@@ -549,7 +546,7 @@ struct Tile16 {
 // candidates kept by every wave took 90 us instead of 30 for 256 x 151936 f32
 // with a list of 8.)
 //
-// Bound by HBM: that call reads its 156 MB at 5.2 TB/s, without a list at 5.7
+// Bound by HBM: that call reads its 156 MB at 5.2 TB/s, without a list at 5.5
 // TB/s.  64 registers, so that 8 waves fit a SIMD (2047 x 32000 f16 with a
 // list of 1: 35 us with 80 registers, 31.6 with 64); the last steps are kept in
 // short loops, since their code comes from L2 when a workgroup first gets there.
@@ -560,7 +557,8 @@ __global__ __launch_bounds__(LT, 8) void logprobs_kernel(LArgs a) {
   __shared__ float s_tmax[TOP ? MAX_TILES : 1];
   __shared__ float s_m[LWAVES], s_s[LWAVES];
   __shared__ uint32_t s_c[LWAVES], s_n[LWAVES], s_sel[TOP_MAX], s_last, s_count, s_bound;
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, wv = tid >> 6;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u;
+  const uint32_t wv = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
   const uint32_t b = blockIdx.x / a.G, g = blockIdx.x % a.G;
   const void* row = (const char*)a.logits + (uint64_t)b * a.stride * Elem<DT>::SZ;
   const uint32_t t0 = g * a.tps, t1 = umin(t0 + a.tps, a.ntiles);
@@ -572,52 +570,70 @@ __global__ __launch_bounds__(LT, 8) void logprobs_kernel(LArgs a) {
   const bool chosen = tok < a.V;
   const float lt = chosen ? raw_logit<DT>(row, tok) : __builtin_huge_valf();
 
+  // NaN counts as -inf.  The maximum and the comparisons leave it out by
+  // themselves, and the sum shows it; only then, or where -inf is what is
+  // compared with, are a tile's logits replaced.  (16-bit logits are bound by
+  // these operations as much as by memory: with each NaN replaced and the counts
+  // kept by lanes, 512 x 128256 bf16 took 33.7 us instead of 29.7.)
+  const bool lowest = lt == NEG_INF;
   float m = NEG_INF, s = 0.0f;
-  uint32_t before = 0;
+  uint32_t before = 0;  // the wave's
   for (; t < t1; t += LWAVES) {
-    float x[16];
+    float x[16], mx, m2, sum;
     in.values(t, a.V, x);
     if (t + LWAVES < t1) in.request(row, t + LWAVES, a.V);
-    float mx = x[0];
+    auto tile = [&]() {
+      mx = x[0];
 #pragma unroll
-    for (uint32_t i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
+      for (uint32_t i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
+      float y[16], my = mx;
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i) y[i] = x[i];
+      if (DT & SOFTCAP) {
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i)  // (a masked token stays one)
+          y[i] = x[i] == NEG_INF ? NEG_INF : cap_f32<DT>(x[i], a.sc_m1, a.sc_cap);
+        my = y[0];
+#pragma unroll
+        for (uint32_t i = 1; i < 16; ++i) my = fmaxf(my, y[i]);
+      }
+      m2 = fmaxf(m, my);
+      const float mm = m2 == NEG_INF ? 0.0f : m2;
+      sum = m2 > m ? s * exp_diff(m, mm) : s;  // (0 the first time)
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i) sum += exp_diff(y[i], mm);
+    };
+    tile();
+    if (lowest || __any(!(sum == sum))) {
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i)
+        if (!(x[i] == x[i])) x[i] = NEG_INF;
+      tile();
+    }
+    m = m2;
+    s = sum;
     if (TOP) {
       const float w = wave_max(mx);
       if (lane == 0) s_tmax[t - t0] = w;
     }
     if (chosen) {
-      if (t * TILE + TILE <= tok) {
+      auto count = [&](auto comes_before) {
 #pragma unroll
-        for (uint32_t i = 0; i < 16; ++i) before += x[i] >= lt ? 1u : 0u;
-      } else if (t * TILE > tok) {
-#pragma unroll
-        for (uint32_t i = 0; i < 16; ++i) before += x[i] > lt ? 1u : 0u;
-      } else {
-#pragma unroll
-        for (uint32_t i = 0; i < 16; ++i)
-          before += x[i] > lt || (x[i] == lt && Tile16<DT>::index(t, i) < tok) ? 1u : 0u;
-      }
+        for (uint32_t i = 0; i < 16; ++i) before += (uint32_t)__popcll(__ballot(comes_before(i)));
+      };
+      if (t * TILE + TILE <= tok)
+        count([&](uint32_t i) { return x[i] >= lt; });
+      else if (t * TILE > tok)
+        count([&](uint32_t i) { return x[i] > lt; });
+      else
+        count([&](uint32_t i) {
+          return x[i] > lt || (x[i] == lt && Tile16<DT>::index(t, i) < tok);
+        });
     }
-    if (DT & SOFTCAP) {
-#pragma unroll
-      for (uint32_t i = 0; i < 16; ++i)  // (a masked token stays one)
-        x[i] = x[i] == NEG_INF ? NEG_INF : cap_f32<DT>(x[i], a.sc_m1, a.sc_cap);
-      mx = x[0];
-#pragma unroll
-      for (uint32_t i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
-    }
-    if (mx > m) {
-      s *= exp_diff(m, mx);  // (0 the first time)
-      m = mx;
-    }
-    const float mm = m == NEG_INF ? 0.0f : m;
-#pragma unroll
-    for (uint32_t i = 0; i < 16; ++i) s += exp_diff(x[i], mm);
   }
   // the wave's, then the workgroup's share
   const float wm = wave_max(m);
   s = wave_tree_sum(m == NEG_INF ? 0.0f : s * exp_diff(m, wm));
-  before = bcast63u(wave_incl_scan(before));
   if (lane == 0) {
     s_m[wv] = wm;
     s_s[wv] = s;
@@ -750,7 +766,8 @@ __global__ __launch_bounds__(LT, 8) void logprobs_kernel(LArgs a) {
   auto gather = [&](const float (&x)[16], uint32_t tt) {
     uint32_t mine = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < 16; ++i) mine |= x[i] >= least ? 1u << i : 0u;
+    for (uint32_t i = 0; i < 16; ++i)  // (a NaN is none below -inf)
+      mine |= least == NEG_INF || x[i] >= least ? 1u << i : 0u;
     while (mine) {  // (few: the logit is read again, which keeps this code short)
       const uint32_t e = Tile16<DT>::index(tt, (uint32_t)__builtin_ctz(mine));
       mine &= mine - 1;

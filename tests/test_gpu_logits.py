@@ -445,6 +445,43 @@ def test_logprobs_masked_rows(sampler, V):
     assert torch.isnan(r.logprobs[6]) and r.logprobs[2].item() == -np.inf
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("softcap", [0.0, 20.0])
+def test_logprobs_nan_of_any_kind(sampler, dtype, softcap):
+    """Quiet and signalling NaN of both signs: single ones, whole tiles of
+    them, and rows with little else, read as -inf wherever they stand."""
+    B, V = 9, 9001
+    lg = np.random.default_rng(12).normal(0, 3, (B, V)).astype(np.float32)
+    x = dev(lg, torch.float32).to(DT[dtype])
+    bits = x.view(torch.int32 if dtype == "f32" else torch.int16)
+    kinds = {"f32": [0x7F800001, 0x7FC00000, -0x7FFFFF, -1], "bf16": [0x7F81, 0x7FC0, -0x7F, -1],
+             "f16": [0x7C01, 0x7E00, -0x3FF, -1]}[dtype]
+    for i, k in enumerate(kinds):
+        bits[0, 5 + 977 * i] = k
+        bits[1, 1000 + i:4000:4] = k
+        bits[2, 17 + i::5] = k  # every fifth token is left
+        bits[3, i::4] = k
+    bits[3, 4242] = bits[4, 4242]  # one token is left
+    bits[4, 8990:] = kinds[0]
+    x[5, :4096] = float("-inf")
+    bits[5, 100:200] = kinds[0]
+    vals = x.double().cpu().numpy()
+    assert np.isnan(vals[3]).sum() == V - 1
+    tokens = np.array([5, 2000, 17, 4242, 8999, 150, 3, 9000, 0])
+    lp, rank, order, tol = expect_logprobs(vals, tokens, 6, softcap)
+    r = sampler.logprobs(x, dev(tokens), top_n=6, softcap=softcap)
+    torch.cuda.synchronize()
+    at = np.arange(B)
+    assert np.array_equal(r.ranks.cpu().numpy(), rank[at, tokens])
+    assert np.array_equal(r.top_ids.cpu().numpy(), order)
+    for got, want, t in ((r.logprobs, lp[at, tokens], tol[at, tokens]),
+                         (r.top_logprobs, np.take_along_axis(lp, order, 1), np.take_along_axis(tol, order, 1))):
+        got = got.double().cpu().numpy()
+        inf = np.isinf(want)
+        assert np.array_equal(got[inf], want[inf])
+        assert (np.abs(got[~inf] - want[~inf]) <= t[~inf]).all()
+
+
 def test_logprobs_tokens_past_the_vocabulary(sampler):
     lg = torch.zeros(3, 100, device="cuda:0")
     r = sampler.logprobs(lg, dev([100, -1, 5]), vocab=100)
