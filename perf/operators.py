@@ -519,8 +519,11 @@ def _update_plain(s):
     refs.copy_(ref[:N])
     lengths.copy_(torch.where(go, new, cur))
     table.copy_(tab)
-    # the copies: rows without one copy a page onto itself
+    # the copies: rows without one repeat the first of them, so that no page is
+    # written in two ways (page 0 onto itself if no row has one)
     a, b = torch.where(cp, last, 0), torch.where(cp, dst, 0)
+    k = cp.long().argmax(0, keepdim=True)
+    a, b = torch.where(cp, a, a[k]), torch.where(cp, b, b[k])
     for p in s["pools"]:
         p.index_copy_(0, b, p[a])
     return {"granted": (~refused).int(), "lengths": lengths, "refs": refs, "table": table, "pools": s["pools"]}
