@@ -278,8 +278,11 @@ int llmk_verify_batch(llmk_sampler* s, uint32_t batch, uint32_t vocab, const uin
  *   v not allowed by the row's mask: x = -inf;
  *   temperature > 1e-5: x /= temperature (sampler.rs:150-157).
  * Each step is one f32 operation, as in llmk_sample_batch: without a softcap
- * the f32 output sampled at temperature 1 with no penalties gives the tokens
- * that the logits give with them.  The result is rounded once, to out_dtype.
+ * the f32 output gives llmk_sample_batch, with no penalties, the tokens that
+ * the logits give with them, at temperature 1 for the rows divided here and at
+ * temperature 0 for the greedy ones (temperature <= 1e-5, sampler.rs:40-50):
+ * those are not divided, and at temperature 1 they would be drawn from.
+ * The result is rounded once, to out_dtype.
  * NaN stays NaN.  (The softcap of 16-bit logits is computed in f32 here and
  * not rounded to 16 bits between its steps as llmk_sample_batch does.)
  *

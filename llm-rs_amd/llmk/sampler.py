@@ -596,7 +596,9 @@ class HipSampler:
                        stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
         """llmk_process_logits: softcap, logit bias, penalties, allow-mask and
         temperature of every row, into `out` ([B, >= V], float32 or the logits'
-        dtype; lb.logits itself: in place), by default a new float32 tensor."""
+        dtype; lb.logits itself: in place), by default a new float32 tensor.
+        Sample from it at temperature 1, and at 0 for greedy rows (temperature
+        <= 1e-5), which are left undivided."""
         if out is None:
             _logits_rows("logits", lb.logits)
             out = _output(stream, lb.logits.shape[0], _vocab(lb.logits, lb.vocab),

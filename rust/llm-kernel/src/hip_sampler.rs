@@ -392,7 +392,9 @@ impl HipSampler {
     }
 
     /// Processed logits (softcap, logit bias, penalties, allow-mask,
-    /// temperature), as `llmk_process_logits` documents.
+    /// temperature), as `llmk_process_logits` documents.  Sample from them at
+    /// temperature 1, and at 0 for greedy rows (temperature <= 1e-5), which
+    /// are left undivided.
     ///
     /// # Safety
     /// As `sample_batch`.
