@@ -285,6 +285,9 @@ int llmk_verify_batch(llmk_sampler* s, uint32_t batch, uint32_t vocab, const uin
  * The result is rounded once, to out_dtype.
  * NaN stays NaN.  (The softcap of 16-bit logits is computed in f32 here and
  * not rounded to 16 bits between its steps as llmk_sample_batch does.)
+ * A softcap takes infinite logits to +-softcap, here and in llmk_sample_batch:
+ * a token that the logits hold at -inf can be sampled again after it.  Tokens
+ * are banned behind the softcap, by allow_mask or a bias of -inf.
  *
  * A row whose sequence is >= sequences, whose mask_index is >= mask_rows or
  * one of whose parameters is not finite is filled with NaN and raises
@@ -347,8 +350,11 @@ int llmk_process_logits(llmk_sampler* s, const llmk_process_logits_args* args,
 
 /* Log-probabilities of a batch of rows (what an OpenAI-style `logprobs`
  * answer holds; no function of the reference has it).  With x = the logit as
- * f32 (softcapped as in llmk_process_logits, -inf staying -inf), m = max x and S = sum
- * exp(x - m), both held in f32: log p(v) = (x_v - m) - log S.  Tokens are
+ * f32 (softcapped as in llmk_process_logits, but for -inf, which stays -inf: a
+ * banned token has no probability here, whatever the softcap), m = max x and S = sum
+ * exp(x - m), both held in f32: log p(v) = (x_v - m) - log S.  For logits that
+ * hold no -inf these are, to f32 accuracy, the log-probabilities of
+ * llmk_process_logits' output with that softcap alone.  Tokens are
  * ordered by (raw logit descending, index ascending); NaN is read as -inf.
  *   out_logprobs[b] = log p(tokens[b]), out_ranks[b] = tokens before it in
  *   the order (0: the likeliest);

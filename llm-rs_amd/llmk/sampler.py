@@ -616,7 +616,9 @@ class HipSampler:
                  top_n: int = 0, softcap: float = 0.0, vocab: Optional[int] = None,
                  stream: Optional[torch.cuda.Stream] = None) -> Logprobs:
         """llmk_logprobs: log-probability and rank of tokens[b] in row b, and
-        the row's top_n likeliest tokens (ties: the lower id first)."""
+        the row's top_n likeliest tokens (ties: the lower id first).  Logits of
+        -inf stay -inf through a softcap here (process_logits and sample_batch
+        take them to -softcap)."""
         a = _lib.LogprobsArgs()
         a.dtype = _logits_rows("logits", logits)
         self._same_device(logits)

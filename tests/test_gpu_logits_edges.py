@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import llmk
-from test_gpu_logits import Case, dev, rows_on_device, sampler  # noqa: F401
+from test_gpu_logits import Case, dev, expect_logprobs, rows_on_device, sampler  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +51,44 @@ def test_greedy_rows_are_sampled_from_processed_logits_at_temperature_0(sampler,
     assert torch.equal(drawn[~greedy], fused.tokens[~greedy])
     assert not torch.equal(drawn[greedy], best[greedy])
     assert sampler.status() == 0
+
+
+@pytest.mark.parametrize("dtype,out", [("f32", "f32"), ("bf16", "f32"), ("bf16", "same"), ("f16", "same")])
+def test_infinite_logits_under_a_softcap(sampler, dtype, out):  # noqa: F811
+    """process_logits takes them to +-softcap, as the sampling call does, and a
+    mask or a bias of -inf bans behind it; logprobs keeps -inf; for logits
+    without it the two agree."""
+    B, V, cap = 2, 5000, 30.0
+    lg = np.random.default_rng(50).normal(0, 20, (B, V)).astype(np.float32)
+    lg[:, [0, 700]], lg[:, [1, 4999]], lg[:, [2, 3]] = np.inf, -np.inf, -np.inf
+    _, view, vals = rows_on_device(lg, dtype)
+    mask = np.full((B, (V + 31) // 32), -1, np.int32)
+    mask[:, 0] = ~np.int32(1 << 2)
+    lb = llmk.LogitsBatch(logits=view, softcap=cap, allow_mask=dev(mask), bias_offsets=dev([0, 1, 2]),
+                          bias_tokens=dev([3, 3]), bias_values=dev([-np.inf, -np.inf], torch.float32))
+    odt = torch.float32 if out == "f32" else view.dtype
+    x = torch.empty(B, V, dtype=odt, device="cuda:0")
+    sampler.process_logits(lb, out=x)
+    assert (x[:, [0, 700]] == cap).all() and (x[:, [1, 4999]] == -cap).all()
+    assert (x[:, [2, 3]] == -np.inf).all() and torch.isfinite(x[:, 4:]).all()
+    # the sampling call's probability of a token at -inf is that of -softcap
+    u = dev([0.5, 0.5], torch.float32)
+    d = sampler.sample_batch(llmk.DeviceBatch(logits=view, softcap=cap, uniforms=u), out_cap=V)
+    for b in range(B):
+        n = int(d.count[b])
+        assert n == V and 1 in d.ids[b, n - 4:].tolist() and d.probs[b, n - 1].item() > 0
+    # tokens 0 and 700 lie at +inf, the lowest ones at -inf
+    r = sampler.logprobs(view, dev([0, 1]), top_n=4, softcap=cap)
+    assert r.top_ids[:, :2].tolist() == [[0, 700]] * 2 and torch.isfinite(r.top_logprobs).all()
+    assert r.logprobs[0].item() == r.top_logprobs[0, 0].item() and r.logprobs[1].item() == -np.inf
+    view[:, [1, 2, 3, 4999]] = -50.0
+    tok = dev([17, 700])
+    one = sampler.logprobs(view, tok, top_n=8, softcap=cap)
+    y = sampler.process_logits(llmk.LogitsBatch(logits=view, softcap=cap))
+    two = sampler.logprobs(y, tok)
+    # both from the same capped values, in sums of another order where the types
+    # differ: each is within the bound for those values, so 2 of them apart
+    yv = y.double().cpu().numpy()
+    _, _, _, tol = expect_logprobs(yv, None, 0, 0.0)
+    off = (one.logprobs.double() - two.logprobs.double()).abs().cpu().numpy()
+    assert (off <= 2 * tol[[0, 1], [17, 700]]).all()
