@@ -330,7 +330,8 @@ typedef struct {
   const uint32_t* extra_count;
   const uint32_t* extra_tokens;
   /* Logit biases per sequence, CSR: bias_offsets[sequences + 1].  A list
-   * holds at most 2^31 pairs; ids >= vocab are ignored.  NULL = none. */
+   * holds at most 2^31 pairs, of which several may have one token; ids >=
+   * vocab are ignored.  NULL = none. */
   const uint32_t* bias_offsets;
   const uint32_t* bias_tokens;
   const float* bias_values;

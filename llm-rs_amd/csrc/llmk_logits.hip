@@ -172,9 +172,11 @@ constexpr uint32_t TOUCHED = 2048;  // tokens listed per segment (below)
 // logit of the segment: how often its token occurs, less one (all ones:
 // never).  A segment is small enough for a word per logit, so this needs no
 // table, no hash and no limit on a history.  A row with biases first uses the
-// words for those: each token's bias, or, where a token is listed more than
-// once, its first place in the list, from which on its biases are summed in
-// listing order, whatever order threads run in.
+// words for those: each token's bias, or, where the segment has a token that is
+// listed more than once, its biases' sum, which the thread that holds its logit
+// adds up from the list in its order: work in proportion to the list (64 x
+// 151936 f32 with 20000 biases 76 us, 150 with one of them repeated in a row,
+// 234 with half of them; a walk down the list per token took 34 ms and 76 ms).
 //
 // Bound by HBM without lists (512 x 128256 bf16 to bf16 47 us, 5.5 TB/s).  With
 // them by the steps before the last logit can be written: extents, tokens,
@@ -196,7 +198,8 @@ template <int DT, int OT, uint32_t N, bool TOUCHED_ONLY>
 __global__ __launch_bounds__(PT, 8) void process_kernel(PArgs a) {
   extern __shared__ uint32_t psm[];
   __shared__ uint16_t s_list[TOUCHED_ONLY ? TOUCHED : 1];
-  __shared__ uint32_t s_listed, s_twice;
+  __shared__ uint32_t s_listed, s_twice, s_here[PT / WAVE];
+  __shared__ u2v s_pair[TOUCHED_ONLY ? 1 : PT];
   // 16 bytes a lane from memory or, where the results are wider, to it: then a
   // wave's stores fill lines (512 x 128257 bf16 to f32 75 us; 83 with 16 bytes
   // read a lane, whose 32 bytes go out in two halves).
@@ -293,40 +296,56 @@ __global__ __launch_bounds__(PT, 8) void process_kernel(PArgs a) {
     lds_barrier();
   }
   if (nb && !TOUCHED_ONLY) {
-    for (uint32_t j = tid; j < nb; j += PT) {
-      const uint32_t t = (j == tid ? bt0 : G(bt)[j]) - lo;
-      const uint32_t v = j == tid ? bv0 : __float_as_uint(G(bv)[j]);
+    auto place = [&](uint32_t t, uint32_t v) {
       if (t < n && __hip_atomic_exchange(cnt + t, v == EMPTY ? 0x7fc00000u : v, __ATOMIC_RELAXED,
                                          __HIP_MEMORY_SCOPE_WORKGROUP) != EMPTY)
         s_twice = 1;
-    }
+    };
+    if (tid < nb) place(bt0 - lo, bv0);  // (waves without a pair wait for no load)
+    for (uint32_t j = PT + tid; j < nb; j += PT)
+      place(G(bt)[j] - lo, G((const uint32_t*)bv)[j]);
     lds_barrier();
-    const bool twice = s_twice != 0;
-    if (twice) {  // the first place of each token instead of its bias
+    if (s_twice != 0) {
+      // Each token's sum instead: PT pairs at a time, those of the segment in
+      // listing order, by the threads that hold their logits.
+      LDS uint32_t* here = (LDS uint32_t*)s_here;
+      LDS u2v* pair = (LDS u2v*)s_pair;
+      const uint32_t wv = tid >> 6;
       clear();
-      lds_barrier();
-      for (uint32_t j = tid; j < nb; j += PT) {
-        const uint32_t t = (j == tid ? bt0 : G(bt)[j]) - lo;
-        if (t < n)
-          __hip_atomic_fetch_min(cnt + t, j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+      for (uint32_t j0 = 0; j0 < nb; j0 += PT) {
+        const uint32_t j = j0 + tid, t = j < nb ? G(bt)[j] - lo : EMPTY;
+        const uint32_t v = t < n ? G((const uint32_t*)bv)[j] : 0u;
+        const uint64_t who = __ballot(t < n);
+        if ((tid & 63u) == 0) here[wv] = (uint32_t)__popcll(who);
+        lds_barrier();
+        uint32_t at = lanes_below(who), all = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < PT / WAVE; ++i) {
+          at += i < wv ? here[i] : 0u;
+          all += here[i];
+        }
+        if (t < n) pair[at] = u2v{t, v};
+        lds_barrier();
+        all = (uint32_t)__builtin_amdgcn_readfirstlane((int)all);
+        for (uint32_t i = 0; i < all; ++i) {
+          const u2v p = pair[i];
+          if (p[0] / W % PT != tid) continue;
+          const uint32_t m = cnt[p[0]];
+          const float sum = m == EMPTY ? __uint_as_float(p[1])
+                                       : __uint_as_float(m) + __uint_as_float(p[1]);
+          cnt[p[0]] = sum == sum ? __float_as_uint(sum) : 0x7fc00000u;
+        }
+        lds_barrier();  // the pairs are read
       }
-      lds_barrier();
     }
 #pragma unroll
     for (uint32_t h = 0; h < N; h += 4) {
       const uint32_t at = ((h / W) * PT + tid) * W + h % W;
       const u4v m = *(LDS u4v*)(cnt + at);
+      if ((m[0] & m[1] & m[2] & m[3]) != EMPTY)  // for the counts
+        *(LDS u4v*)(cnt + at) = u4v{EMPTY, EMPTY, EMPTY, EMPTY};
 #pragma unroll
-      for (uint32_t k = 0; k < 4; ++k) {
-        add[h + k] = m[k] == EMPTY ? 0.0f : __uint_as_float(m[k]);
-        if (m[k] == EMPTY) continue;
-        cnt[at + k] = EMPTY;  // for the counts
-        if (twice) {
-          add[h + k] = G(bv)[m[k]];
-          for (uint32_t j = m[k] + 1; j < nb; ++j)
-            if (G(bt)[j] == lo + at + k) add[h + k] += G(bv)[j];
-        }
-      }
+      for (uint32_t k = 0; k < 4; ++k) add[h + k] = m[k] == EMPTY ? 0.0f : __uint_as_float(m[k]);
     }
     lds_barrier();
   }

@@ -92,3 +92,77 @@ def test_infinite_logits_under_a_softcap(sampler, dtype, out):  # noqa: F811
     _, _, _, tol = expect_logprobs(yv, None, 0, 0.0)
     off = (one.logprobs.double() - two.logprobs.double()).abs().cpu().numpy()
     assert (off <= 2 * tol[[0, 1], [17, 700]]).all()
+
+
+@pytest.mark.parametrize("B,V,dtype", [(1, 100, "f32"), (3, 5003, "bf16"), (2, 40000, "f32"), (260, 17000, "f16")])
+def test_biases_listed_more_than_once_are_summed_in_listing_order(sampler, B, V, dtype):  # noqa: F811
+    """Bit for bit the f32 sums in the list's order, on logits of zero: tokens
+    listed once, twice on both sides of a multiple of 256 and hundreds of times,
+    ids past the vocabulary, whole lists repeated, lists without a repetition."""
+    rng = np.random.default_rng(V)
+    lists = []
+    for b in range(B):
+        m = int(rng.integers(1, 600))
+        t = rng.choice(V + 50, min(m, V))
+        kind = b % 4
+        if kind == 0:
+            t = np.concatenate([t, t])
+        elif kind == 1:
+            t = np.concatenate([t, np.full(300, t[0]), t[:2]])
+        elif kind == 2 and m > 3:
+            t = np.concatenate([[t[0]], np.arange(V, V + 255), [t[0]], t, [t[1]]])
+        lists.append((t, (rng.normal(0, 1, len(t)) * 10.0 ** rng.integers(-6, 7, len(t))).astype(np.float32)))
+    want = np.zeros((B, V), np.float32)
+    for b, (t, v) in enumerate(lists):
+        seen = set()
+        for i, x in zip(t, v):
+            if i < V:
+                want[b, i] = want[b, i] + x if i in seen else x
+                seen.add(i)
+    off = np.concatenate([[0], np.cumsum([len(t) for t, _ in lists])])
+    lg = torch.zeros(B, V, dtype={"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[dtype],
+                     device="cuda:0")
+    lb = llmk.LogitsBatch(logits=lg, bias_offsets=dev(off), bias_tokens=dev(np.concatenate([t for t, _ in lists])),
+                          bias_values=dev(np.concatenate([v for _, v in lists]), torch.float32))
+    got = sampler.process_logits(lb).cpu().numpy()
+    assert np.array_equal(got, want)
+
+
+def test_nan_biases_of_any_kind_on_a_token_listed_twice(sampler):  # noqa: F811
+    """The NaN whose bits are all ones among them, first and last in a list."""
+    bits = np.array([0xFFFFFFFF, 0x7FFFFFFF, 0x7F800001, 0xFFFFFFFF], np.uint32).view(np.float32)
+    vals = np.array([bits[0], 1.0, 2.0, bits[1], bits[2], 3.0, bits[3], bits[3], 4.0, 5.0], np.float32)
+    lb = llmk.LogitsBatch(logits=torch.ones(1, 3000, device="cuda:0"), bias_offsets=dev([0, 10]),
+                          bias_tokens=dev([5, 5, 8, 8, 2100, 2100, 2900, 2900, 40, 40]),
+                          bias_values=torch.as_tensor(vals).cuda())
+    g = sampler.process_logits(lb)[0].cpu()
+    assert torch.isnan(g[[5, 8, 2100, 2900]]).all() and int(torch.isnan(g).sum()) == 4
+    assert g[40] == 10.0 and g[0] == 1.0 and g[2999] == 1.0
+
+
+@pytest.mark.parametrize("B", [1, 64])
+def test_a_repeated_bias_costs_in_proportion_to_the_list(sampler, B):  # noqa: F811
+    """20000 pairs with one token listed twice, or half of them, against the
+    same number of distinct ones."""
+    V, n = 151936, 20000
+    rng = np.random.default_rng(0)
+    lg, out = torch.randn(B, V, device="cuda:0"), torch.empty(B, V, device="cuda:0")
+
+    def time(repeated):
+        tok = np.stack([rng.choice(V, n, replace=False) for _ in range(B)])
+        tok[:, n - repeated:] = tok[:, :repeated]
+        lb = llmk.LogitsBatch(logits=lg, bias_offsets=dev(np.arange(B + 1) * n), bias_tokens=dev(tok.reshape(-1)),
+                              bias_values=torch.randn(B * n, device="cuda:0"))
+        best = float("inf")
+        for _ in range(5):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            sampler.process_logits(lb, out=out)
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    once = time(0)
+    # walking the list anew for every listed token takes several hundred times as long
+    assert time(1) < 40 * once and time(n // 2) < 40 * once
