@@ -293,7 +293,8 @@ int llmk_verify_batch(llmk_sampler* s, uint32_t batch, uint32_t vocab, const uin
  * one of whose parameters is not finite is filled with NaN and raises
  * LLMK_STATUS_INVALID_PARAMS. */
 typedef struct {
-  /* logits[b * row_stride + v], rows at any element offset. */
+  /* logits[b * row_stride + v], rows at any element offset;
+   * batch * row_stride <= 2^55. */
   const void* logits;
   int32_t dtype; /* llmk_dtype */
   uint32_t batch;

@@ -888,12 +888,14 @@ static bool known_dtype(int32_t dt) {
 }
 
 // Checks what both operators ask of their rows of logits.
-static int check_rows(const void* p, int32_t dtype, uint32_t vocab, uint64_t stride,
-                      const char* what) {
+static int check_rows(const void* p, int32_t dtype, uint32_t batch, uint32_t vocab,
+                      uint64_t stride, const char* what) {
   if (!known_dtype(dtype))
     return fail(LLMK_ERR_INVALID_ARGUMENT,
                 std::string(what) + ": dtype must be LLMK_F32, LLMK_BF16 or LLMK_F16");
   if (stride < vocab) return fail(LLMK_ERR_INVALID_ARGUMENT, std::string(what) + ": stride < vocab");
+  if (batch && stride > (1ull << 55) / batch)  // (so that no offset in bytes overflows)
+    return fail(LLMK_ERR_CAPACITY, std::string(what) + ": batch * stride above 2^55");
   if (((uintptr_t)p % (dtype == LLMK_F32 ? 4 : 2)) != 0)
     return fail(LLMK_ERR_ALIGNMENT, std::string(what) + " must be aligned to their elements");
   return LLMK_OK;
@@ -927,8 +929,8 @@ extern "C" int llmk_process_logits(llmk_sampler* s, const llmk_process_logits_ar
   if (in->vocab == 0) return fail(LLMK_ERR_EMPTY_LOGITS, "Empty logits passed to process_logits");
   if (!in->logits || !in->out)
     return fail(LLMK_ERR_INVALID_ARGUMENT, "logits and out are required");
-  int rc = check_rows(in->logits, in->dtype, in->vocab, in->row_stride, "logits");
-  if (rc == LLMK_OK) rc = check_rows(in->out, in->out_dtype, in->vocab, in->out_stride, "out");
+  int rc = check_rows(in->logits, in->dtype, in->batch, in->vocab, in->row_stride, "logits");
+  if (rc == LLMK_OK) rc = check_rows(in->out, in->out_dtype, in->batch, in->vocab, in->out_stride, "out");
   if (rc == LLMK_OK) rc = check_softcap(in->softcap);
   if (rc != LLMK_OK) return rc;
   if (in->out_dtype != LLMK_F32 && in->out_dtype != in->dtype)
@@ -1030,7 +1032,7 @@ extern "C" int llmk_logprobs(llmk_sampler* s, const llmk_logprobs_args* in, void
   if (!in) return fail(LLMK_ERR_INVALID_ARGUMENT, "args is NULL");
   if (in->vocab == 0) return fail(LLMK_ERR_EMPTY_LOGITS, "Empty logits passed to logprobs");
   if (!in->logits) return fail(LLMK_ERR_INVALID_ARGUMENT, "logits are required");
-  int rc = check_rows(in->logits, in->dtype, in->vocab, in->row_stride, "logits");
+  int rc = check_rows(in->logits, in->dtype, in->batch, in->vocab, in->row_stride, "logits");
   if (rc == LLMK_OK) rc = check_softcap(in->softcap);
   if (rc != LLMK_OK) return rc;
   if (!in->tokens && in->top_n == 0)

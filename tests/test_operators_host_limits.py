@@ -1,0 +1,54 @@
+"""The operators' host checks at the ends of their arguments' ranges, without a
+GPU.  Each call runs in a process of its own: what a check lets through must not
+end the caller's."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+CALL = """
+import ctypes, sys
+sys.path.insert(0, {pkg!r})
+from llmk import _lib
+lib = _lib.load()
+handle = ctypes.cast(ctypes.create_string_buffer(4096), ctypes.c_void_p)
+a = _lib.{struct}()
+for k, v in {fields!r}.items():
+    setattr(a, k, v)
+rc = lib.{function}(handle, ctypes.byref(a), None)
+print(rc, _lib.last_error())
+"""
+
+P = 0x10000
+PROCESS = dict(logits=P, dtype=0, batch=2, vocab=100, row_stride=100, out=P * 16, out_dtype=0, out_stride=100)
+LOGPROBS = dict(logits=P, dtype=0, batch=2, vocab=8, row_stride=8, tokens=P, out_logprobs=P)
+
+
+def call(function, struct, fields):
+    code = CALL.format(pkg=os.path.join(ROOT, "llm-rs_amd"), struct=struct, function=function, fields=fields)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, (r.returncode, r.stderr[-500:])
+    rc, _, message = r.stdout.strip().partition(" ")
+    return int(rc), message
+
+
+def process(**kw):
+    return call("llmk_process_logits", "ProcessLogitsArgs", dict(PROCESS, **kw))
+
+
+def logprobs(**kw):
+    return call("llmk_logprobs", "LogprobsArgs", dict(LOGPROBS, **kw))
+
+
+@pytest.mark.parametrize("kw", [dict(row_stride=2**62, out=P + 4, out_stride=2**62),
+                                dict(row_stride=2**63, out=P + 4, out_stride=2**63),
+                                dict(row_stride=2**54 + 1), dict(out_stride=2**54 + 1)])
+def test_strides_whose_bytes_overflow_are_refused(kw):
+    rc, message = process(**kw)
+    assert rc == -3 and "2^55" in message
+    if "out_stride" not in kw:
+        rc, message = logprobs(**kw)
+        assert rc == -3 and "2^55" in message
