@@ -883,6 +883,10 @@ __global__ __launch_bounds__(LT, 8) void logprobs_kernel(LArgs a) {
 // ===========================================================================
 using namespace llmk;
 
+// The most threads that a launch's grid has along x: HIP takes a grid by its
+// threads, in 32 bits.
+constexpr uint32_t GRID_THREADS = 0xffffffffu;
+
 static bool known_dtype(int32_t dt) {
   return dt == LLMK_F32 || dt == LLMK_BF16 || dt == LLMK_F16;
 }
@@ -1044,7 +1048,6 @@ extern "C" int llmk_logprobs(llmk_sampler* s, const llmk_logprobs_args* in, void
     return fail(LLMK_ERR_INVALID_ARGUMENT, "top_n needs out_top_ids and out_top_logprobs");
   if (in->vocab > MAX_TILES * TILE) return fail(LLMK_ERR_CAPACITY, "vocab above 2^20");
   if (in->batch == 0) return LLMK_OK;
-  HIPCHK(hipSetDevice(s->device));
   LArgs a;
   a.logits = in->logits;
   a.stride = in->row_stride;
@@ -1071,6 +1074,7 @@ extern "C" int llmk_logprobs(llmk_sampler* s, const llmk_logprobs_args* in, void
   // 43.8.
   const uint32_t lt = !in->top_n ? 256 : (a.ntiles < 40 ? (a.B <= 256 ? 512 : 256)
                                                         : (a.B <= 256 ? 1024 : 512));
+  if (a.B > GRID_THREADS / lt) return fail(LLMK_ERR_CAPACITY, "batch too large for one call");
   // Segments per row: 4096 waves, four on each SIMD, while each has a tile.
   const uint32_t pool = s->max_batch > MAX_WGS ? s->max_batch : MAX_WGS, waves = lt / WAVE;
   uint32_t g = (4096 / waves + a.B - 1) / a.B;
@@ -1080,10 +1084,9 @@ extern "C" int llmk_logprobs(llmk_sampler* s, const llmk_logprobs_args* in, void
   if (a.B > s->max_batch || (uint64_t)a.B * g > pool) g = 1;
   a.tps = (a.ntiles + g - 1) / g;
   a.G = (a.ntiles + a.tps - 1) / a.tps;
-  const uint64_t blocks = (uint64_t)a.B * a.G;
-  if (blocks > 0x7fffffffu) return fail(LLMK_ERR_CAPACITY, "batch above 2^31 - 1");
+  HIPCHK(hipSetDevice(s->device));
   auto launch = [&](auto kern) {
-    hipLaunchKernelGGL(kern, dim3((uint32_t)blocks), dim3(lt), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(kern, dim3(a.B * a.G), dim3(lt), 0, (hipStream_t)stream, a);
   };
 #define LLMK_LOGPROBS(DT)                                              \
   do {                                                                 \

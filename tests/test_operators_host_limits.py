@@ -52,3 +52,12 @@ def test_strides_whose_bytes_overflow_are_refused(kw):
     if "out_stride" not in kw:
         rc, message = logprobs(**kw)
         assert rc == -3 and "2^55" in message
+
+
+# 256 threads a row, or 512 where a row has 40 tiles of 1024 logits and a top list
+@pytest.mark.parametrize("kw", [dict(batch=2**32 - 1), dict(batch=2**32 - 512), dict(batch=2**24),
+                                dict(batch=2**23, vocab=40960, row_stride=40960, top_n=1, out_top_ids=P,
+                                     out_top_logprobs=P)])
+def test_logprobs_of_more_rows_than_a_grid_holds(kw):
+    rc, message = logprobs(**kw)
+    assert rc == -3 and "too large" in message
