@@ -346,7 +346,8 @@ typedef struct {
 } llmk_process_logits_args;
 
 /* Enqueued on hip_stream; allocates nothing and uses no workspace of the
- * handle, whose maxima do not bound batch and vocab. */
+ * handle, whose maxima do not bound batch and vocab.  batch * ceil(vocab / 4096)
+ * < 2^24. */
 int llmk_process_logits(llmk_sampler* s, const llmk_process_logits_args* args,
                         void* hip_stream);
 
@@ -382,7 +383,8 @@ typedef struct {
 
 /* Enqueued on hip_stream; allocates nothing; uses the handle's workspace
  * (stream order, like llmk_sample_batch).  Batches above the handle's
- * max_batch run with one workgroup per row. */
+ * max_batch run with one workgroup per row.  batch < 2^24; < 2^23 with a top
+ * list and vocab above 39 * 1024. */
 int llmk_logprobs(llmk_sampler* s, const llmk_logprobs_args* args, void* hip_stream);
 
 /* A cache in pages: what the scheduler's block allocator keeps on the host

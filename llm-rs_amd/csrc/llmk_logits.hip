@@ -970,7 +970,8 @@ extern "C" int llmk_process_logits(llmk_sampler* s, const llmk_process_logits_ar
   const uint32_t seg = (large ? big : small) * PT;
   const uint32_t nseg = (in->vocab + seg - 1) / seg;
   const uint64_t blocks = (uint64_t)in->batch * nseg;
-  if (blocks > 0x7fffffffu) return fail(LLMK_ERR_CAPACITY, "batch * vocab too large for one call");
+  if (blocks > GRID_THREADS / PT)
+    return fail(LLMK_ERR_CAPACITY, "batch * vocab too large for one call");
   HIPCHK(hipSetDevice(s->device));
   PArgs a;
   a.in = in->logits;

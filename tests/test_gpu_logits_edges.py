@@ -166,3 +166,22 @@ def test_a_repeated_bias_costs_in_proportion_to_the_list(sampler, B):  # noqa: F
     once = time(0)
     # walking the list anew for every listed token takes several hundred times as long
     assert time(1) < 40 * once and time(n // 2) < 40 * once
+
+
+def test_as_many_rows_as_a_grid_holds(sampler):  # noqa: F811
+    """2^24 - 1 rows, a workgroup each: every row is served."""
+    B = 2**24 - 1
+    lg = torch.randn(B, 2, device="cuda:0")
+    x = sampler.process_logits(llmk.LogitsBatch(logits=lg, temperature=torch.full((B,), 2.0, device="cuda:0")))
+    assert torch.equal(x, lg / 2)
+    r = sampler.logprobs(lg, torch.ones(B, dtype=torch.int32, device="cuda:0"))
+    assert torch.equal(r.ranks, (lg[:, 0] >= lg[:, 1]).int())
+    # two terms, a difference, a logarithm below 1 and a last difference
+    want = lg[:, 1].double() - torch.logsumexp(lg.double(), 1)
+    tol = 2.0 ** -24 * (32 + 4 * (lg[:, 0] - lg[:, 1]).abs().double())
+    assert bool(((r.logprobs.double() - want).abs() <= tol).all())
+    more = torch.empty(B + 1, 2, device="cuda:0")
+    with pytest.raises(llmk.SamplerError, match="too large"):
+        sampler.process_logits(llmk.LogitsBatch(logits=more))
+    with pytest.raises(llmk.SamplerError, match="too large"):
+        sampler.logprobs(more, top_n=1)

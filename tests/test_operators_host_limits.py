@@ -61,3 +61,11 @@ def test_strides_whose_bytes_overflow_are_refused(kw):
 def test_logprobs_of_more_rows_than_a_grid_holds(kw):
     rc, message = logprobs(**kw)
     assert rc == -3 and "too large" in message
+
+
+@pytest.mark.parametrize("kw", [dict(batch=2**24, vocab=8, row_stride=8, out_stride=8, out=2**40),
+                                dict(batch=2**22, vocab=4 * 4096, row_stride=2**15, out_stride=2**15, out=2**50),
+                                dict(batch=2**32 - 1, vocab=1, row_stride=1, out_stride=1, out=2**40)])
+def test_process_logits_of_more_segments_than_a_grid_holds(kw):
+    rc, message = process(**kw)
+    assert rc == -3 and "too large" in message
