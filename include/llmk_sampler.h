@@ -306,7 +306,7 @@ typedef struct {
   void* out;
   int32_t out_dtype;
   uint64_t out_stride;
-  float softcap; /* 0 = off */
+  float softcap; /* 0 = off, or 2^-126 and above */
   /* The sequence of each row, [batch]: rows of one sequence share its
    * parameters, history and biases (a speculative chain's positions).
    * NULL: row b is sequence b, and sequences is not read. */

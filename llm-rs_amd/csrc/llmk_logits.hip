@@ -907,6 +907,8 @@ static int check_rows(const void* p, int32_t dtype, uint32_t batch, uint32_t voc
 static int check_softcap(float c) {
   if (!(c >= 0.0f) || !(c < __builtin_huge_valf()))
     return fail(LLMK_ERR_INVALID_ARGUMENT, "softcap must be finite and >= 0 (0 = off)");
+  if (c > 0.0f && c < 0x1p-126f)  // 1 / softcap overflows, and a logit of 0 would be NaN
+    return fail(LLMK_ERR_INVALID_ARGUMENT, "softcap below 2^-126");
   return LLMK_OK;
 }
 

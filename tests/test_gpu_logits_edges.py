@@ -185,3 +185,13 @@ def test_as_many_rows_as_a_grid_holds(sampler):  # noqa: F811
         sampler.process_logits(llmk.LogitsBatch(logits=more))
     with pytest.raises(llmk.SamplerError, match="too large"):
         sampler.logprobs(more, top_n=1)
+
+
+def test_the_smallest_softcap(sampler):  # noqa: F811
+    """2^-126: a logit of 0 stays 0, the others become +-softcap."""
+    cap = 2.0 ** -126
+    lg = dev([[0.0, -0.0, 3.0, -1e30, cap * 32, -np.inf]], torch.float32)
+    x = sampler.process_logits(llmk.LogitsBatch(logits=lg, softcap=cap))
+    assert x[0].tolist() == [0.0, 0.0, cap, -cap, cap, -cap]
+    r = sampler.logprobs(lg, dev([0]), top_n=5, softcap=cap)
+    assert torch.isfinite(r.logprobs).all() and torch.isfinite(r.top_logprobs).all()

@@ -69,3 +69,10 @@ def test_logprobs_of_more_rows_than_a_grid_holds(kw):
 def test_process_logits_of_more_segments_than_a_grid_holds(kw):
     rc, message = process(**kw)
     assert rc == -3 and "too large" in message
+
+
+@pytest.mark.parametrize("cap", [1e-45, 2.0**-129, 1.1754942e-38])
+def test_softcaps_whose_reciprocal_may_overflow_are_refused(cap):
+    for f in (process, logprobs):
+        rc, message = f(softcap=cap)
+        assert rc == -1 and "softcap" in message
