@@ -4,8 +4,9 @@
 //! the `hip-sampler` feature.
 
 use std::ffi::c_void;
-use llm_kernel::hip_sampler::{HipSampler, LlmkLogprobsArgs, LlmkPageCache, LlmkProcessLogitsArgs,
-                               LlmkSampleBatchArgs, LLMK_ERR_INVALID_ARGUMENT};
+use llm_kernel::hip_sampler::{pages_work_words, HipSampler, LlmkLogprobsArgs, LlmkPageCache,
+                               LlmkProcessLogitsArgs, LlmkSampleBatchArgs,
+                               LLMK_ERR_INVALID_ARGUMENT};
 
 /// A sampler on `device` for batches up to `max_batch` rows of up to
 /// `max_vocab` logits; null on failure.
@@ -86,6 +87,12 @@ pub unsafe extern "C" fn llm_logprobs(sampler: *mut c_void, args: *const LlmkLog
     }
 }
 
+/// The words of a page cache's work array; 0 where the sizes are refused.
+#[no_mangle]
+pub extern "C" fn llm_pages_work_words(rows: u32, num_pages: u32) -> u64 {
+    pages_work_words(rows, num_pages).unwrap_or(0)
+}
+
 /// One step of a paged cache's rows (see `HipSampler::pages_update`): 0 on
 /// success, else the error code.
 /// # SAFETY: as llm_sample_batch; the cache's arrays are device memory.
@@ -98,6 +105,38 @@ pub unsafe extern "C" fn llm_pages_update(sampler: *mut c_void, cache: *const Ll
     }
     let s = &*(sampler as *const HipSampler);
     match s.pages_update(&*cache, parents, new_lengths, out_granted, stream) {
+        Ok(()) => 0,
+        Err(e) => e.code,
+    }
+}
+
+/// Moves a cache's pages in use to the front (see `HipSampler::pages_compact`):
+/// 0 on success, else the error code.
+/// # SAFETY: as llm_pages_update; `out_map` has `num_pages` entries.
+#[no_mangle]
+pub unsafe extern "C" fn llm_pages_compact(sampler: *mut c_void, cache: *const LlmkPageCache,
+                                           out_map: *mut u32, stream: *mut c_void) -> i32 {
+    if sampler.is_null() || cache.is_null() {
+        return LLMK_ERR_INVALID_ARGUMENT;
+    }
+    match (*(sampler as *const HipSampler)).pages_compact(&*cache, out_map, stream) {
+        Ok(()) => 0,
+        Err(e) => e.code,
+    }
+}
+
+/// Copies page `src[i]` to page `dst[i]` in every pool (see
+/// `HipSampler::pages_copy`): 0 on success, else the error code.
+/// # SAFETY: as llm_sample_batch; every array is device memory.
+#[no_mangle]
+pub unsafe extern "C" fn llm_pages_copy(sampler: *mut c_void, n_pools: u32, pools: *const u64,
+                                        page_bytes: u64, num_pages: u32, n: u32, src: *const u32,
+                                        dst: *const u32, stream: *mut c_void) -> i32 {
+    if sampler.is_null() {
+        return LLMK_ERR_INVALID_ARGUMENT;
+    }
+    let s = &*(sampler as *const HipSampler);
+    match s.pages_copy(n_pools, pools, page_bytes, num_pages, n, src, dst, stream) {
         Ok(()) => 0,
         Err(e) => e.code,
     }
