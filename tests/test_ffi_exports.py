@@ -14,10 +14,11 @@ BINDING = open(os.path.join(ROOT, "rust", "llm-kernel", "src", "hip_sampler.rs")
 
 def parameters(src, name):
     """(name, type) of each parameter of a function, its result and its body."""
-    m = re.search(r"fn %s\(([^)]*)\)\s*->\s*([^{]+?)\s*\{\n(.*?)\n( *)\}\n" % name, src, flags=re.S)
+    m = re.search(r'\n( *)pub (?:unsafe )?(?:extern "C" )?fn %s\(([^)]*)\)\s*->\s*([^{]+?)\s*\{\n(.*?)\n\1\}\n'
+                  % name, src, flags=re.S)
     assert m, name
-    params = [tuple(x.strip() for x in p.split(":")) for p in m.group(1).split(",") if ":" in p]
-    return params, m.group(2), m.group(3)
+    params = [tuple(x.strip() for x in p.split(":")) for p in m.group(2).split(",") if ":" in p]
+    return params, m.group(3), m.group(4)
 
 
 @pytest.mark.parametrize("method", ["process_logits", "logprobs", "pages_update", "pages_compact", "pages_copy"])
