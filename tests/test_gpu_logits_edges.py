@@ -195,3 +195,41 @@ def test_the_smallest_softcap(sampler):  # noqa: F811
     assert x[0].tolist() == [0.0, 0.0, cap, -cap, cap, -cap]
     r = sampler.logprobs(lg, dev([0]), top_n=5, softcap=cap)
     assert torch.isfinite(r.logprobs).all() and torch.isfinite(r.top_logprobs).all()
+
+
+@pytest.mark.parametrize("V", [262144, 262145, 524289, 900001, 2**20])
+@pytest.mark.parametrize("B,n", [(1, 1), (3, 20), (70, 32), (300, 5)])
+def test_logprobs_of_vocabularies_whose_tiles_are_selected_in_groups(sampler, V, B, n):  # noqa: F811
+    """More than 256 tiles of 1024 logits: in groups of two to four, with ties
+    within a group and across groups, rows that hold nothing and little."""
+    if B * V > 10**8:
+        V = V // 8 * 3 + 1  # (as few groups as a row of many needs)
+        V = max(V, 262145)
+    rng = np.random.default_rng(V + B)
+    rows = min(B, 6)
+    lg = rng.normal(0, 3, (rows, V)).astype(np.float32)
+    if rows > 1:
+        lg[1] = np.round(lg[1])
+    if rows > 2:
+        lg[2] = -np.inf
+        lg[2, [V - 1, 5, 2048, 2049, 300000 % V]] = [1.0, 1.0, 0.0, 0.0, 2.0]
+    if rows > 3:
+        lg[3] = np.arange(V) // 1024 % 7
+        lg[4] = np.nan
+        lg[4, V - 3] = -1.0
+        lg[5, ::7] = lg[5].max()
+    many = np.resize(np.arange(rows), B)
+    x = dev(lg, torch.float32)[dev(many).long()]
+    tok = rng.integers(0, V, B)
+    tok[::3] = [np.nanargmax(lg[r]) for r in many[::3]]
+    lp, rank, order, tol = expect_logprobs(lg.astype(np.float64), None, n, 0.0)
+    r = sampler.logprobs(x, dev(tok), top_n=n)
+    assert np.array_equal(r.ranks.cpu().numpy(), rank[many, tok])
+    assert np.array_equal(r.top_ids.cpu().numpy(), order[many])
+    for got, want, t in ((r.logprobs, lp[many, tok], tol[many, tok]),
+                         (r.top_logprobs, np.take_along_axis(lp, order, 1)[many],
+                          np.take_along_axis(tol, order, 1)[many])):
+        got = got.double().cpu().numpy()
+        fin = np.isfinite(want)
+        assert np.array_equal(got[~fin], want[~fin])
+        assert (np.abs(got[fin] - want[fin]) <= t[fin]).all()
