@@ -384,7 +384,9 @@ typedef struct {
 /* Enqueued on hip_stream; allocates nothing; uses the handle's workspace
  * (stream order, like llmk_sample_batch).  Batches above the handle's
  * max_batch run with one workgroup per row.  batch < 2^24; < 2^23 with a top
- * list and vocab above 39 * 1024. */
+ * list and vocab above 39 * 1024.  A top list that has about as many entries as
+ * the row has tiles of 1024 logits, or more, takes several times as long as a
+ * shorter one. */
 int llmk_logprobs(llmk_sampler* s, const llmk_logprobs_args* args, void* hip_stream);
 
 /* A cache in pages: what the scheduler's block allocator keeps on the host

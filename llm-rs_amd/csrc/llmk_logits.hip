@@ -563,7 +563,12 @@ struct Tile16 {
 // maxima of those before it.  So the stream carries no list; the last
 // workgroup reads top_n tiles again and picks from them.  (A list of
 // candidates kept by every wave took 90 us instead of 30 for 256 x 151936 f32
-// with a list of 8.)
+// with a list of 8.)  A row of fewer tiles than that has no bound on the list's
+// last token, and one of about as many has a low one: all or many of its logits
+// are gathered, do not fit, and are read again by the lists that the last lines
+// keep.  That takes several times as long (f32, 64 x 16000 with a list of 8 11 us,
+// of 20 65; 1000 x 5000 with a list of 1 12 us, of 20 96; 64 x 32000 with a list
+// of 20 14 us, of 32 93).
 //
 // Bound by HBM: that call reads its 156 MB at 5.2 TB/s, without a list at 5.5
 // TB/s.  64 registers, so that 8 waves fit a SIMD (2047 x 32000 f16 with a
@@ -774,8 +779,8 @@ __global__ __launch_bounds__(LT, 8) void logprobs_kernel(LArgs a) {
   }
   __syncthreads();
   const uint32_t ns = s_n[0];
-  // Nothing below the bound belongs to the list (if there are top_n groups):
-  // what does not fall below is gathered by all waves.
+  // Nothing below the bound belongs to the list: what does not fall below is
+  // gathered by all waves.  With fewer than top_n groups that is the whole row.
   const float least = s_bound > fkey(NEG_INF) ? funkey(s_bound) : NEG_INF;
   // the selected tiles in turn, a wave each
   auto selected = [&](uint32_t k) {
@@ -831,8 +836,9 @@ __global__ __launch_bounds__(LT, 8) void logprobs_kernel(LArgs a) {
     }
     return;
   }
-  // More than that (rows of equal logits, masked rows with fewer tokens left
-  // than the list holds): by lists that keep the first top_n.
+  // More than that (rows of few tiles for the list's length, rows of equal
+  // logits, masked rows with fewer tokens left than the list holds): by lists that
+  // keep the first top_n.
   __syncthreads();
   LDS uint64_t* list = (LDS uint64_t*)s_list + wv * TLIST;
   uint32_t held = 0;
@@ -1070,11 +1076,16 @@ extern "C" int llmk_logprobs(llmk_sampler* s, const llmk_logprobs_args* in, void
   a.ntiles = (a.V + TILE - 1) / TILE;
   // The workgroup's size only matters to the last steps of a row with a top
   // list, where one workgroup reads tiles again: the more waves the shorter
-  // they take, but the fewer rows a CU holds meanwhile.  Measured with 256,
-  // 512 and 1024 threads: 256 x 151936 f32 top 8: 35.0, 33.0, 30.9 us; 64 x
-  // 50257 f32 top 5: 14.9, 11.9, 11.5; 16 x 32000 f32: 10.8, 9.4, 10.1; 1000 x
-  // 100000 bf16 top 3: 47.2, 43.8, 47.1; 2047 x 32000 f16 top 1: 31.6, 33.4,
-  // 43.8.
+  // they take, but the fewer rows a CU holds meanwhile.  Up to 256 rows each has a
+  // CU to itself, and 1024 threads are as fast as fewer or faster (256 x 152552
+  // bf16 top 5: 256, 512 and 1024 threads 24.3, 22.5, 20.5 us; 64 x 50257 f32 14.9,
+  // 11.9, 11.5), one row more and rows wait for each other (257 x 152552: 25.0,
+  // 25.3, 28.7).  Rows of fewer than 40 tiles have less than three for each of 16
+  // waves, and take one size less: 200 x 39912 f32 16.8, 16.3, 17.2; but 256 x
+  // 20456 15.6, 13.9, 11.3.  Past 256 rows 512 threads for long ones (512 x 102376
+  // f32 43.9, 40.1, 42.8), 256 for short ones, which is right for many (2047 x
+  // 32000 f16 top 1 31.6, 33.4, 43.8) and not for some hundreds (512 x 20456 f32
+  // 18.2, 15.0, 16.2).
   const uint32_t lt = !in->top_n ? 256 : (a.ntiles < 40 ? (a.B <= 256 ? 512 : 256)
                                                         : (a.B <= 256 ? 1024 : 512));
   if (a.B > GRID_THREADS / lt) return fail(LLMK_ERR_CAPACITY, "batch too large for one call");
