@@ -8,14 +8,19 @@ import re
 import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-FFI = open(os.path.join(ROOT, "rust", "llm-ffi", "src", "sampler.rs")).read()
-BINDING = open(os.path.join(ROOT, "rust", "llm-kernel", "src", "hip_sampler.rs")).read()
+FFI = os.path.join(ROOT, "rust", "llm-ffi", "src", "sampler.rs")
+BINDING = os.path.join(ROOT, "rust", "llm-kernel", "src", "hip_sampler.rs")
 
 
-def parameters(src, name):
+def source(path):  # (read by the tests: the module is also imported where the file is not)
+    with open(path) as f:
+        return f.read()
+
+
+def parameters(path, name):
     """(name, type) of each parameter of a function, its result and its body."""
     m = re.search(r'\n( *)pub (?:unsafe )?(?:extern "C" )?fn %s\(([^)]*)\)\s*->\s*([^{]+?)\s*\{\n(.*?)\n\1\}\n'
-                  % name, src, flags=re.S)
+                  % name, source(path), flags=re.S)
     assert m, name
     params = [tuple(x.strip() for x in p.split(":")) for p in m.group(2).split(",") if ":" in p]
     return params, m.group(3), m.group(4)
@@ -34,7 +39,7 @@ def test_each_method_is_exported(method):
     # what is behind a reference is checked before it is read
     for name in ["sampler"] + [n for n, t in want if t.startswith("&")]:
         assert f"{name}.is_null()" in body
-    assert re.search(r'#\[no_mangle\]\npub unsafe extern "C" fn llm_%s\(' % method, FFI)
+    assert re.search(r'#\[no_mangle\]\npub unsafe extern "C" fn llm_%s\(' % method, source(FFI))
 
 
 def test_the_size_of_a_cache_s_work_array_is_exported():
@@ -43,6 +48,6 @@ def test_the_size_of_a_cache_s_work_array_is_exported():
     got, result, body = parameters(FFI, "llm_pages_work_words")
     assert got == want and result == "u64"
     assert "pages_work_words(rows, num_pages).unwrap_or(0)" in body
-    assert re.search(r'#\[no_mangle\]\npub extern "C" fn llm_pages_work_words\(', FFI)
-    used = re.search(r"use llm_kernel::hip_sampler::\{(.*?)\};", FFI, flags=re.S).group(1)
+    assert re.search(r'#\[no_mangle\]\npub extern "C" fn llm_pages_work_words\(', source(FFI))
+    used = re.search(r"use llm_kernel::hip_sampler::\{(.*?)\};", source(FFI), flags=re.S).group(1)
     assert "pages_work_words" in [x.strip() for x in used.split(",")]
